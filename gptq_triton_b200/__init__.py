@@ -10,6 +10,7 @@ from .befalix import BefalixConfig, BefalixEngine, BefalixForCausalLM, load_befa
 from .lifinex import LifinexConfig, LifinexEngine, LifinexForCausalLM, load_lifinex, synthetic_lifinex
 from .llama import DecodeEngine, LlamaConfig, LlamaForCausalLM
 from .loader import autotune_warmup, load_quant, save_quant, synthetic_quantized_llama
+from .paged import PagedPlan, paged_append, paged_attention, paged_plan
 from .registry import ARCHITECTURES, load_model, make_engine
 from .quant_linear import QuantLinear, dequantize, make_quant, qmatmul, triton_matmul4, unpack_qweight, unpack_qzeros
 
@@ -21,6 +22,7 @@ __all__ = [
 	'load_model', 'make_engine', 'ARCHITECTURES',
 	'BefalixConfig', 'BefalixEngine', 'BefalixForCausalLM', 'load_befalix', 'synthetic_befalix',
 	'LifinexConfig', 'LifinexEngine', 'LifinexForCausalLM', 'load_lifinex', 'synthetic_lifinex',
+	'PagedPlan', 'paged_plan', 'paged_append', 'paged_attention',
 	'dequantize', 'unpack_qweight', 'unpack_qzeros',
 	'quant_linear', 'fused_mlp',
 ]

@@ -1,0 +1,95 @@
+"""ctypes binding of libpaged_b200.so (declared in include/paged_b200.h).  Like the other bindings it has no fallback: a missing
+library or a failing kernel raises."""
+from __future__ import annotations
+
+import ctypes
+from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p
+from pathlib import Path
+from typing import Dict, Optional
+
+import torch
+
+from ._lib import GptqB200Error, ptr, register_status_buffer, require_cuda, stream_ptr      # noqa: F401
+
+LIB_PATH = Path(__file__).resolve().parent / 'libpaged_b200.so'
+CONTROL_BYTES = 16384
+MAX_REQUESTS = 8192
+MAX_DIM = 256
+DTYPE_CODE = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+
+_P, _I = c_void_p, c_int
+
+
+class Plan(ctypes.Structure):
+	_fields_ = [(n, _I) for n in ('requests', 'rows', 'table_width', 'page', 'pages', 'pool_size')] + [('table_ld', c_int64)] + [
+		(n, _P) for n in ('past', 'fresh', 'table', 'pool', 'head', 'next_head', 'row_start', 'lens', 'positions', 'slots')] + [
+		(n, _I) for n in ('heads', 'kv_heads', 'dim', 'max_fresh')] + [('work', _P), ('status', _P)]
+
+
+class Append(ctypes.Structure):
+	_fields_ = [(n, _I) for n in ('rows', 'heads', 'kv_heads', 'dim', 'rot', 'max_pos', 'page', 'pages')] + [(n, _P) for n in ('q', 'k', 'v')] + [
+		(n, c_int64) for n in ('q_row', 'q_head', 'k_row', 'k_head', 'v_row', 'v_head')] + [
+		(n, _P) for n in ('cos_t', 'sin_t', 'positions', 'slots', 'q_out', 'k_cache', 'v_cache')] + [
+		(n, c_int64) for n in ('k_page', 'k_kv', 'v_page', 'v_kv')] + [('status', _P)]
+
+
+class Attention(ctypes.Structure):
+	_fields_ = [(n, _I) for n in ('requests', 'rows', 'heads', 'kv_heads', 'dim', 'page', 'pages', 'table_width', 'max_fresh')] + [
+		('table_ld', c_int64), ('scale', c_float), ('q', _P), ('q_row', c_int64), ('q_head', c_int64), ('k_cache', _P), ('v_cache', _P)] + [
+		(n, c_int64) for n in ('k_page', 'k_kv', 'v_page', 'v_kv')] + [(n, _P) for n in ('table', 'row_start', 'lens', 'work', 'out', 'scratch')] + [
+		('scratch_bytes', c_size_t), ('status', _P)]
+
+
+_SIGNATURES = {
+	'paged_version': (c_int, []),
+	'paged_last_cuda_error': (c_int, []),
+	'paged_work_ints': (c_int64, [_I, _I, _I, _I]),
+	'paged_plan': (c_int, [_P, _I, _P]),
+	'paged_append': (c_int, [_P, _I, _P]),
+	'paged_attention_scratch': (c_int64, [_P, _I]),
+	'paged_attention': (c_int, [_P, _I, _P]),
+}
+
+_lib: Optional[ctypes.CDLL] = None
+_control: Dict[int, torch.Tensor] = {}
+
+
+def exported_symbols():
+	"""Names that include/paged_b200.h declares."""
+	return list(_SIGNATURES)
+
+
+def lib() -> ctypes.CDLL:
+	global _lib
+	if _lib is None:
+		if not LIB_PATH.exists():
+			raise ImportError(f'{LIB_PATH} is missing: build it with `python -m gptq_triton_b200.build` (needs nvcc with sm_100a support). '
+							  'There is no CPU or Triton fallback.')
+		l = ctypes.CDLL(str(LIB_PATH))
+		for name, (res, args) in _SIGNATURES.items():
+			fn = getattr(l, name)
+			fn.restype, fn.argtypes = res, args
+		_lib = l
+	return _lib
+
+
+_MESSAGES = {-1: 'invalid argument', -2: 'shape violates a divisibility rule', -3: 'scratch missing or too small', -4: 'pointer or stride misaligned', -5: 'CUDA error', -6: 'not supported'}
+
+
+def check(code: int, what: str):
+	if code != 0:
+		extra = f' (cudaError {lib().paged_last_cuda_error()})' if code == -5 else ''
+		raise (ValueError if code in (-1, -2, -4) else GptqB200Error)(f'{what}: {_MESSAGES.get(code, "unknown error code")}{extra}')
+
+
+def status_ptr(device: torch.device) -> int:
+	"""Address of the status word of the paged operators on `device` (part of _lib.kernel_status())."""
+	index = torch.cuda.current_device() if device.index is None else device.index
+	buf = _control.get(index)
+	if buf is None:
+		if torch.cuda.is_current_stream_capturing():
+			raise GptqB200Error('the first paged operator on a device must run outside of a graph capture: it sets up the status word')
+		buf = _control[index] = torch.zeros(CONTROL_BYTES, dtype=torch.uint8, device=device)
+		torch.cuda.current_stream(device).synchronize()          # (any stream may use it from now on)
+		register_status_buffer(buf)
+	return buf.data_ptr() + CONTROL_BYTES - 4

@@ -2,9 +2,10 @@
 
   libgptq_b200.so    4-bit quantised linear layers, attention and decode kernels   (csrc/*.cu)
   libdense_b200.so   dense-weight layers and latent attention                      (csrc/dense/*.cu)
+  libpaged_b200.so   block tables, rows and attention of a cache in pages          (csrc/paged/*.cu)
   _host.so           layer calls without ctypes, against torch's C++ library       (csrc/host/*.cpp, with g++)
 
-Usage:  python -m gptq_triton_b200.build [--force] [--verbose] [gptq] [dense] [host]
+Usage:  python -m gptq_triton_b200.build [--force] [--verbose] [gptq] [dense] [paged] [host]
 """
 from __future__ import annotations
 
@@ -23,12 +24,14 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / 'csrc'
 LIB = PKG / 'libgptq_b200.so'
 DENSE_LIB = PKG / 'libdense_b200.so'
+PAGED_LIB = PKG / 'libpaged_b200.so'
 HOST_LIB = PKG / '_host.so'
 
 # library -> (output, folder of its sources, further folders whose headers they include)
 TARGETS = {
 	'gptq': (LIB, CSRC, []),
 	'dense': (DENSE_LIB, CSRC / 'dense', [CSRC]),
+	'paged': (PAGED_LIB, CSRC / 'paged', [CSRC]),
 	'host': (HOST_LIB, CSRC / 'host', []),
 }
 

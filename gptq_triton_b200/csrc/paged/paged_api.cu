@@ -1,0 +1,68 @@
+// C ABI of the paged-cache library: checks of arguments and the choice of kernels.
+#include <new>
+
+#include "paged.cuh"
+
+namespace gptq {
+thread_local int g_last_cuda_error = 0;
+}
+
+using namespace gptq;
+
+namespace {
+
+bool known(int dtype) { return dtype == PG_BF16 || dtype == PG_F32 || dtype == PG_F16; }
+int size_of(int dtype) { return dtype == PG_F32 ? 4 : 2; }
+bool heads_ok(int heads, int kv_heads) { return kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && heads <= 65535; }
+// heads and pages start on 16 bytes
+bool steps_ok(int64_t a, int64_t b, int dtype) { return a >= 0 && b >= 0 && a * size_of(dtype) % 16 == 0 && b * size_of(dtype) % 16 == 0; }
+
+}   // namespace
+
+extern "C" {
+
+int paged_version(void) { return 100; }
+int paged_last_cuda_error(void) { return g_last_cuda_error; }
+
+int64_t paged_work_ints(int requests, int rows, int heads, int kv_heads) {
+	if (requests < 0 || rows < 0 || !heads_ok(heads, kv_heads)) return -1;
+	return 16;
+}
+
+int paged_plan(const paged_plan_t *p, int dtype, void *stream) {
+	if (!p || !known(dtype) || p->requests < 0 || p->requests > PAGED_MAX_REQUESTS || p->rows < 0 || p->page < 1 || p->pages < 0 || p->table_width < 1 || p->table_ld < p->table_width ||
+		!heads_ok(p->heads, p->kv_heads) || !p->row_start || !p->work || !p->status || p->max_fresh < 0)
+		return GPTQ_ERR_INVALID;
+	if (p->requests && (!p->past || !p->fresh || !p->table || !p->lens)) return GPTQ_ERR_INVALID;
+	if (p->rows && (!p->positions || !p->slots)) return GPTQ_ERR_INVALID;
+	if (p->pool && (!p->head || !p->next_head || p->head == p->next_head || p->pool_size < 0)) return GPTQ_ERR_INVALID;
+	return pg_plan_launch(*p, dtype, (cudaStream_t)stream);
+}
+
+int paged_append(const paged_append_t *p, int dtype, void *stream) {
+	if (!p || !known(dtype) || p->rows < 0 || !heads_ok(p->heads, p->kv_heads) || p->dim < 1 || p->rot < 0 || p->rot > p->dim || p->rot % 2 || p->page < 1 || p->pages < 0 || !p->status)
+		return GPTQ_ERR_INVALID;
+	if (p->rows == 0) return GPTQ_OK;
+	if (!p->q || !p->k || !p->v || !p->q_out || !p->k_cache || !p->v_cache || !p->slots || (p->rot && (!p->cos_t || !p->sin_t || !p->positions || p->max_pos < 1))) return GPTQ_ERR_INVALID;
+	return pg_append_launch(*p, dtype, (cudaStream_t)stream);
+}
+
+int64_t paged_attention_scratch(const paged_attention_t *p, int dtype) {
+	if (!p || !known(dtype)) return -1;
+	return 16;
+}
+
+int paged_attention(const paged_attention_t *p, int dtype, void *stream) {
+	if (!p || !known(dtype) || p->requests < 0 || p->requests > PAGED_MAX_REQUESTS || p->rows < 0 || !heads_ok(p->heads, p->kv_heads) || p->page < 1 || p->pages < 0 || p->table_width < 1 ||
+		p->table_ld < p->table_width || !(p->scale > 0.f) || !(p->scale <= 3.4e38f) || !p->status)
+		return GPTQ_ERR_INVALID;
+	if (p->dim < 1 || p->dim > PAGED_MAX_DIM || p->dim % 8) return GPTQ_ERR_SHAPE;
+	if (p->requests == 0 || p->rows == 0) return GPTQ_OK;
+	if (!p->q || !p->k_cache || !p->v_cache || !p->table || !p->row_start || !p->lens || !p->work || !p->out) return GPTQ_ERR_INVALID;
+	if (!steps_ok(p->k_page, p->k_kv, dtype) || !steps_ok(p->v_page, p->v_kv, dtype) || !steps_ok(p->q_row, p->q_head, dtype) || !aligned16(p->q) || !aligned16(p->k_cache) || !aligned16(p->v_cache) ||
+		!aligned16(p->out))
+		return GPTQ_ERR_ALIGN;
+	return pg_attend_simple(*p, dtype, (cudaStream_t)stream);
+}
+
+}   // extern "C"

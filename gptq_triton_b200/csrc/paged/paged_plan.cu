@@ -1,0 +1,177 @@
+// Block tables, slot maps, positions and row offsets of a step from the request lengths, and the distribution of the attention's work.
+//
+// Every CTA scans the lengths of all requests into shared memory for itself (two sums per request: rows and pages taken), which is
+// cheaper than a second launch or a barrier over the grid; then CTA 0 lays out the attention's work, the others write pages and rows.
+// A row finds its request by bisection in shared memory.  Table entries that are read (pages of old tokens) and written (pages taken
+// now) are different ones, so the order of the CTAs does not matter, and a second run over the same inputs writes the same.
+// The bytes are nothing; what counts is the chain launch - lengths - scan - table entry - store.
+#include "paged.cuh"
+
+namespace gptq {
+
+namespace {
+
+constexpr int PL_THREADS = 1024;
+
+// sums that stop at a limit (associative for values of at least 0)
+__device__ __forceinline__ int add_to(int a, int b, int limit) { return min(a + b, limit); }
+constexpr int PL_LIMIT = 1 << 30;
+
+// exclusive scan over the CTA of two values per thread; returns the totals in (ta, tb).  s: 66 ints of shared memory
+__device__ __forceinline__ void scan2(int &a, int &b, int limit_a, int limit_b, int &ta, int &tb, int *s) {
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+	int x = a, y = b;
+#pragma unroll
+	for (int d = 1; d < 32; d <<= 1) {
+		const int u = __shfl_up_sync(0xffffffffu, x, d), v = __shfl_up_sync(0xffffffffu, y, d);
+		if (lane >= d) {
+			x = add_to(x, u, limit_a);
+			y = add_to(y, v, limit_b);
+		}
+	}
+	__syncthreads();
+	if (lane == 31) {
+		s[warp] = x;
+		s[32 + warp] = y;
+	}
+	__syncthreads();
+	int px = s[lane], py = s[32 + lane];          // (32 warps)
+#pragma unroll
+	for (int d = 1; d < 32; d <<= 1) {
+		const int u = __shfl_up_sync(0xffffffffu, px, d), v = __shfl_up_sync(0xffffffffu, py, d);
+		if (lane >= d) {
+			px = add_to(px, u, limit_a);
+			py = add_to(py, v, limit_b);
+		}
+	}
+	ta = __shfl_sync(0xffffffffu, px, 31);
+	tb = __shfl_sync(0xffffffffu, py, 31);
+	const int bx = __shfl_sync(0xffffffffu, px, (warp + 31) & 31), by = __shfl_sync(0xffffffffu, py, (warp + 31) & 31);
+	int ex = __shfl_up_sync(0xffffffffu, x, 1), ey = __shfl_up_sync(0xffffffffu, y, 1);
+	if (lane == 0) ex = ey = 0;
+	a = warp ? add_to(bx, ex, limit_a) : ex;
+	b = warp ? add_to(by, ey, limit_b) : ey;
+}
+
+// the last i in [0, n) with v[i] <= x (v ascending, v[0] <= x)
+__device__ __forceinline__ int find(const int *v, int n, int x) {
+	int lo = 0, hi = n;
+	while (hi - lo > 1) {
+		const int mid = (lo + hi) >> 1;
+		if (v[mid] <= x) lo = mid;
+		else hi = mid;
+	}
+	return lo;
+}
+
+struct Lengths { int past, fresh, old, full; };
+
+__device__ __forceinline__ Lengths lengths_of(const paged_plan_t &p, int r, int &bad) {
+	Lengths l;
+	l.past = __ldg(p.past + r);
+	l.fresh = __ldg(p.fresh + r);
+	if (l.past < 0 || l.past > PL_LIMIT || l.fresh < 0 || l.fresh > PL_LIMIT / 2) {
+		bad |= PAGED_BAD_INDEX;
+		l.past = min(max(l.past, 0), PL_LIMIT);
+		l.fresh = min(max(l.fresh, 0), PL_LIMIT / 2);
+	}
+	l.old = (l.past + p.page - 1) / p.page;
+	l.full = (l.past + l.fresh + p.page - 1) / p.page;
+	if (p.pool == nullptr) l.full = l.old = 0;          // the table is complete
+	return l;
+}
+
+__global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, int tiles) {
+	extern __shared__ int pl_smem[];
+	__shared__ int s_scan[64];
+	int *s_start = pl_smem, *s_off = pl_smem + p.requests + 1;
+	const int tid = threadIdx.x, R = p.requests;
+	int bad = 0, rows = 0, taken = 0;
+	for (int base = 0; base < R; base += PL_THREADS) {
+		const int r = base + tid;
+		int a = 0, b = 0;
+		if (r < R) {
+			const Lengths l = lengths_of(p, r, bad);
+			a = min(l.fresh, p.rows + 1);
+			b = l.full - l.old;
+		}
+		int ta, tb;
+		scan2(a, b, p.rows + 1, PL_LIMIT, ta, tb, s_scan);
+		if (r < R) {
+			s_start[r] = min(add_to(rows, a, p.rows + 1), p.rows);
+			s_off[r] = add_to(taken, b, PL_LIMIT);
+		}
+		rows = add_to(rows, ta, p.rows + 1);
+		taken = add_to(taken, tb, PL_LIMIT);
+	}
+	if (tid == 0) s_start[R] = min(rows, p.rows);
+	if (rows > p.rows) bad |= PAGED_NO_ROOM;
+	__syncthreads();
+	const int head = p.pool ? __ldg(p.head) : 0, used = s_start[R];
+	if (p.pool && (head < 0 || head > p.pool_size || taken > p.pool_size - head)) bad |= head < 0 || head > p.pool_size ? PAGED_BAD_INDEX : PAGED_NO_ROOM;
+
+	// the page that entry c of request r names; -1: none
+	auto page_of = [&](int r, int c, int old) {
+		int id;
+		if (p.pool && c >= old) {
+			const long long at = (long long)head + s_off[r] + (c - old);
+			id = at >= 0 && at < p.pool_size ? __ldg(p.pool + at) : -1;
+		} else {
+			id = c < p.table_width ? p.table[(int64_t)r * p.table_ld + c] : -1;
+		}
+		return id;
+	};
+
+	if (blockIdx.x == 0) {
+		for (int r = tid; r < R; r += PL_THREADS) {
+			const Lengths l = lengths_of(p, r, bad);
+			p.row_start[r] = s_start[r];
+			p.lens[r] = l.past + l.fresh;
+		}
+		if (tid == 0) {
+			p.row_start[R] = used;
+			if (p.pool) *p.next_head = min(max(head, 0), p.pool_size) + min(taken, p.pool_size - min(max(head, 0), p.pool_size));
+		}
+	} else {
+		// pages that are taken now: a warp per request
+		const int warps = (gridDim.x - 1) * (PL_THREADS / 32), lane = tid & 31;
+		if (p.pool)
+			for (int r = (blockIdx.x - 1) * (PL_THREADS / 32) + (tid >> 5); r < R; r += warps) {
+				const Lengths l = lengths_of(p, r, bad);
+				if (l.full > p.table_width) bad |= PAGED_NO_ROOM;
+				for (int c = l.old + lane; c < min(l.full, p.table_width); c += 32) p.table[(int64_t)r * p.table_ld + c] = page_of(r, c, l.old);
+			}
+		for (int m = (blockIdx.x - 1) * PL_THREADS + tid; m < p.rows; m += (gridDim.x - 1) * PL_THREADS) {
+			int pos = 0;
+			int64_t slot = -1;
+			if (m < used) {
+				const int r = find(s_start, R, m);
+				const int past = min(max(__ldg(p.past + r), 0), PL_LIMIT);
+				pos = past + m - s_start[r];
+				const int c = pos / p.page;
+				const int id = page_of(r, c, (past + p.page - 1) / p.page);
+				if (c >= p.table_width) bad |= PAGED_NO_ROOM;
+				else if (id >= 0 && id < p.pages) slot = (int64_t)id * p.page + (pos - c * p.page);
+				else bad |= PAGED_BAD_INDEX;
+			}
+			p.positions[m] = pos;
+			p.slots[m] = slot;
+		}
+	}
+	if (bad) atomicOr(p.status, bad);
+}
+
+}   // namespace
+
+int pg_plan_launch(const paged_plan_t &p, int dtype, cudaStream_t stream) {
+	const int tiles = pg_tiles_serve(dtype, p.dim, p.page, p.max_fresh, p.heads, p.kv_heads);
+	const size_t smem = (size_t)(2 * p.requests + 1) * sizeof(int);
+	static_assert((2 * PAGED_MAX_REQUESTS + 1) * sizeof(int) + 4096 <= 227 * 1024, "shared memory");
+	if (smem > 48 * 1024 - 4096)
+		if (int rc = cuda_status(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))) return rc;
+	const int fill = (int)((p.rows + (int64_t)PL_THREADS - 1) / PL_THREADS), ctas = 1 + (fill < 1 ? 1 : fill > 295 ? 295 : fill);
+	plan_kernel<<<ctas, PL_THREADS, smem, stream>>>(p, tiles);
+	return cuda_status(cudaGetLastError());
+}
+
+}   // namespace gptq
