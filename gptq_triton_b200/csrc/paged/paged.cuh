@@ -36,10 +36,14 @@ constexpr int PG_ROWS = 16, PG_KEYS = 64, PG_SLOTS = 296;
 constexpr int PG_TILE = 256, PG_TILE_KEYS = 128, PG_TILE_SLOTS = 148;
 
 struct PgList {                        // of one of the two kernels; behind it in `work`: starts, entries, order
-	int entries, per, total;            // total: units of all key heads
+	int entries;
 	int whole;                          // slots take whole tiles by `order` instead (tile kernel)
+	int64_t per, total;                 // units of all key heads
 };
-struct PgEntry { int request, tile, blocks, first; };          // blocks of keys that the tile sees; first: units of the entries before, per key head
+struct PgEntry {
+	int request, tile, blocks, first;   // blocks of keys that the tile sees; units of the entries before, per key head
+	int row, fresh, len, seen;          // first row and new tokens of the request, its tokens, those that the tile's last row sees
+};
 struct PgStart { int entry, kv, block, pad; };                 // entry -1: nothing to do
 
 struct PgWork {
@@ -62,9 +66,9 @@ inline __host__ __device__ PgWork pg_work(int32_t *base, int requests, int rows,
 	w.starts[1] = reinterpret_cast<PgStart *>(base + at);
 	at += 4 * (PG_TILE_SLOTS + 1);
 	w.entries[0] = reinterpret_cast<PgEntry *>(base + at);
-	at += 4 * (int64_t)w.cap[0];
+	at += 8 * (int64_t)w.cap[0];
 	w.entries[1] = reinterpret_cast<PgEntry *>(base + at);
-	at += 4 * (int64_t)w.cap[1];
+	at += 8 * (int64_t)w.cap[1];
 	w.order = base + at;
 	w.ints = at + w.cap[1];
 	return w;
@@ -74,8 +78,46 @@ inline bool pg_tiles_serve(int dtype, int dim, int page, int max_fresh, int head
 	return false;
 }
 
+// cp.async of 16 bytes; `bytes` 0 writes zeros and reads nothing
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, int bytes) {
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+	float r;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+	return r;
+}
+constexpr float PG_LOG2E = 1.44269504088896341f;
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<bf16>(float lo, float hi) {
+	__nv_bfloat162 a = __floats2bfloat162_rn(lo, hi);
+	return *reinterpret_cast<uint32_t *>(&a);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+	__half2 a = __floats2half2_rn(lo, hi);
+	return *reinterpret_cast<uint32_t *>(&a);
+}
+// D(16x8) += A(16x16, row) * B(16x8, col); fragment ownership as in mma16816
+template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { mma16816(d, a[0], a[1], a[2], a[3], b0, b1); }
+template <> __device__ __forceinline__ void mma16<bf16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+	asm volatile(
+		"mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+		: "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+		: "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+	asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+	asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
 int pg_plan_launch(const paged_plan_t &p, int dtype, cudaStream_t stream);
 int pg_append_launch(const paged_append_t &p, int dtype, cudaStream_t stream);
+int64_t pg_rows_scratch(const paged_attention_t &p);
+int pg_rows_launch(const paged_attention_t &p, int dtype, cudaStream_t stream);          // fp16, bf16
 int pg_attend_simple(const paged_attention_t &p, int dtype, cudaStream_t stream);
 
 }   // namespace gptq

@@ -25,17 +25,18 @@ int paged_version(void) { return 100; }
 int paged_last_cuda_error(void) { return g_last_cuda_error; }
 
 int64_t paged_work_ints(int requests, int rows, int heads, int kv_heads) {
-	if (requests < 0 || rows < 0 || !heads_ok(heads, kv_heads)) return -1;
-	return 16;
+	if (requests < 0 || requests > PAGED_MAX_REQUESTS || rows < 0 || !heads_ok(heads, kv_heads) || (int64_t)rows * (heads / kv_heads) >= (int64_t)1 << 31) return -1;
+	return pg_work(nullptr, requests, rows, heads, kv_heads).ints;
 }
 
 int paged_plan(const paged_plan_t *p, int dtype, void *stream) {
 	if (!p || !known(dtype) || p->requests < 0 || p->requests > PAGED_MAX_REQUESTS || p->rows < 0 || p->page < 1 || p->pages < 0 || p->table_width < 1 || p->table_ld < p->table_width ||
-		!heads_ok(p->heads, p->kv_heads) || !p->row_start || !p->work || !p->status || p->max_fresh < 0)
+		!heads_ok(p->heads, p->kv_heads) || !p->row_start || !p->work || !p->status || p->max_fresh < 0 || paged_work_ints(p->requests, p->rows, p->heads, p->kv_heads) < 0)
 		return GPTQ_ERR_INVALID;
 	if (p->requests && (!p->past || !p->fresh || !p->table || !p->lens)) return GPTQ_ERR_INVALID;
 	if (p->rows && (!p->positions || !p->slots)) return GPTQ_ERR_INVALID;
 	if (p->pool && (!p->head || !p->next_head || p->head == p->next_head || p->pool_size < 0)) return GPTQ_ERR_INVALID;
+	if (!aligned16(p->work)) return GPTQ_ERR_ALIGN;
 	return pg_plan_launch(*p, dtype, (cudaStream_t)stream);
 }
 
@@ -48,8 +49,8 @@ int paged_append(const paged_append_t *p, int dtype, void *stream) {
 }
 
 int64_t paged_attention_scratch(const paged_attention_t *p, int dtype) {
-	if (!p || !known(dtype)) return -1;
-	return 16;
+	if (!p || !known(dtype) || p->dim < 1 || p->dim > PAGED_MAX_DIM) return -1;
+	return dtype == PG_F32 ? 16 : pg_rows_scratch(*p);
 }
 
 int paged_attention(const paged_attention_t *p, int dtype, void *stream) {
@@ -62,7 +63,9 @@ int paged_attention(const paged_attention_t *p, int dtype, void *stream) {
 	if (!steps_ok(p->k_page, p->k_kv, dtype) || !steps_ok(p->v_page, p->v_kv, dtype) || !steps_ok(p->q_row, p->q_head, dtype) || !aligned16(p->q) || !aligned16(p->k_cache) || !aligned16(p->v_cache) ||
 		!aligned16(p->out))
 		return GPTQ_ERR_ALIGN;
-	return pg_attend_simple(*p, dtype, (cudaStream_t)stream);
+	if (dtype == PG_F32) return pg_attend_simple(*p, dtype, (cudaStream_t)stream);
+	if (!p->scratch || !aligned16(p->scratch) || (int64_t)p->scratch_bytes < pg_rows_scratch(*p)) return GPTQ_ERR_WORKSPACE;
+	return pg_rows_launch(*p, dtype, (cudaStream_t)stream);
 }
 
 }   // extern "C"

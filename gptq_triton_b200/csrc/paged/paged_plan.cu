@@ -81,6 +81,71 @@ __device__ __forceinline__ Lengths lengths_of(const paged_plan_t &p, int r, int 
 	return l;
 }
 
+// What the attention sees of a request is at most what its table can name.
+__device__ __forceinline__ int length_seen(const paged_plan_t &p, const Lengths &l) { return (int)min((int64_t)l.past + l.fresh, min((int64_t)p.table_width * p.page, (int64_t)PL_LIMIT)); }
+
+constexpr int PL_KEEP = 4096;          // units before an entry that are kept in shared memory for the search
+
+// The work list of one kernel.  s_tiles [R + 1]: tiles of the requests before; s_first: PL_KEEP ints.
+__device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, const int *s_tiles, int *s_first, int *s_scan, PgWork w) {
+	const int tid = threadIdx.x, R = p.requests, tile_rows = kind ? PG_TILE : PG_ROWS, keys = kind ? PG_TILE_KEYS : PG_KEYS, group = p.heads / p.kv_heads;
+	const int slots = kind ? PG_TILE_SLOTS : PG_SLOTS;
+	const int E = min(s_tiles[R], w.cap[kind]);
+	int units = 0;
+	for (int base = 0; base < E; base += PL_THREADS) {
+		const int e = base + tid;
+		PgEntry x = {};
+		int bad = 0, n = 0, none = 0;
+		if (e < E) {
+			x.request = find(s_tiles, R, e);
+			x.tile = e - s_tiles[x.request];
+			x.row = s_start[x.request];
+			x.fresh = s_start[x.request + 1] - x.row;
+			x.len = length_seen(p, lengths_of(p, x.request, bad));
+			const int last = (int)((min((int64_t)x.fresh * group, (int64_t)(x.tile + 1) * tile_rows) - 1) / group);
+			x.seen = min(max(x.len - x.fresh + last + 1, 0), x.len);
+			n = x.blocks = max((x.seen + keys - 1) / keys, 1);
+		}
+		int total, unused;
+		scan2(n, none, PL_LIMIT, PL_LIMIT, total, unused, s_scan);
+		if (e < E) {
+			x.first = add_to(units, n, PL_LIMIT);
+			w.entries[kind][e] = x;
+			if (e < PL_KEEP) s_first[e] = x.first;
+		}
+		units = add_to(units, total, PL_LIMIT);
+	}
+	__syncthreads();
+	const int64_t total = (int64_t)units * p.kv_heads, per = max((total + slots - 1) / slots, (int64_t)(kind ? 2 : 2));
+	if (tid == 0) w.list[kind] = PgList{E, 0, per, total};
+	for (int c = tid; c <= slots; c += PL_THREADS) {
+		const int64_t u = c * per;
+		PgStart s = {-1, 0, 0, 0};
+		if (u < total) {
+			const int x = (int)(u / p.kv_heads);
+			int e;
+			if (E <= PL_KEEP) {
+				e = find(s_first, E, x);
+			} else {
+				int lo = 0, hi = E;
+				while (hi - lo > 1) {
+					const int mid = (lo + hi) >> 1;
+					if (w.entries[kind][mid].first <= x) lo = mid;
+					else hi = mid;
+				}
+				e = lo;
+			}
+			const int n = w.entries[kind][e].blocks;
+			const int64_t rest = u - (int64_t)w.entries[kind][e].first * p.kv_heads;
+			s.entry = e;
+			s.kv = (int)(rest / n);
+			s.block = (int)(rest % n);
+		}
+		w.starts[kind][c] = s;
+	}
+	__syncthreads();
+}
+
 __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, int tiles) {
 	extern __shared__ int pl_smem[];
 	__shared__ int s_scan[64];
@@ -126,12 +191,41 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, 
 		for (int r = tid; r < R; r += PL_THREADS) {
 			const Lengths l = lengths_of(p, r, bad);
 			p.row_start[r] = s_start[r];
-			p.lens[r] = l.past + l.fresh;
+			p.lens[r] = length_seen(p, l);
+			if (p.lens[r] < l.past + l.fresh) bad |= PAGED_NO_ROOM;
 		}
 		if (tid == 0) {
 			p.row_start[R] = used;
 			if (p.pool) *p.next_head = min(max(head, 0), p.pool_size) + min(taken, p.pool_size - min(max(head, 0), p.pool_size));
 		}
+		int *s_few = s_off + R + 1, *s_many = s_few + R + 1, *s_first = s_many + R + 1;
+		const int group = p.heads / p.kv_heads;
+		int few = 0, many = 0;
+		for (int base = 0; base < R; base += PL_THREADS) {
+			const int r = base + tid;
+			int a = 0, b = 0;
+			if (r < R) {
+				const int64_t n = (int64_t)(s_start[r + 1] - s_start[r]) * group;
+				if (tiles && n > PG_ROWS) b = (int)((n + PG_TILE - 1) / PG_TILE);
+				else a = (int)((n + PG_ROWS - 1) / PG_ROWS);
+			}
+			int ta, tb;
+			scan2(a, b, PL_LIMIT, PL_LIMIT, ta, tb, s_scan);
+			if (r < R) {
+				s_few[r] = few + a;
+				s_many[r] = many + b;
+			}
+			few += ta;
+			many += tb;
+		}
+		if (tid == 0) {
+			s_few[R] = few;
+			s_many[R] = many;
+		}
+		__syncthreads();
+		const PgWork w = pg_work(p.work, R, p.rows, p.heads, p.kv_heads);
+		lay_out(p, 0, s_start, s_few, s_first, s_scan, w);
+		if (tiles) lay_out(p, 1, s_start, s_many, s_first, s_scan, w);
 	} else {
 		// pages that are taken now: a warp per request
 		const int warps = (gridDim.x - 1) * (PL_THREADS / 32), lane = tid & 31;
@@ -165,8 +259,8 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, 
 
 int pg_plan_launch(const paged_plan_t &p, int dtype, cudaStream_t stream) {
 	const int tiles = pg_tiles_serve(dtype, p.dim, p.page, p.max_fresh, p.heads, p.kv_heads);
-	const size_t smem = (size_t)(2 * p.requests + 1) * sizeof(int);
-	static_assert((2 * PAGED_MAX_REQUESTS + 1) * sizeof(int) + 4096 <= 227 * 1024, "shared memory");
+	const size_t smem = (size_t)(4 * (p.requests + 1) + PL_KEEP) * sizeof(int);
+	static_assert((4 * (PAGED_MAX_REQUESTS + 1) + PL_KEEP) * sizeof(int) + 4096 <= 227 * 1024, "shared memory");
 	if (smem > 48 * 1024 - 4096)
 		if (int rc = cuda_status(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))) return rc;
 	const int fill = (int)((p.rows + (int64_t)PL_THREADS - 1) / PL_THREADS), ctas = 1 + (fill < 1 ? 1 : fill > 295 ? 295 : fill);

@@ -54,7 +54,325 @@ __global__ void __launch_bounds__(128) simple_kernel(const paged_attention_t p) 
 		if (lane + 32 * i < p.dim) reinterpret_cast<T *>(p.out)[((int64_t)m * p.heads + h) * p.dim + lane + 32 * i] = PgElem<T>::put(pos < 0 ? 0.f : o[i] / sum);
 }
 
+// ---- fp16 and bf16 ------------------------------------------------------------------------------------------------------------
+// Keys and values stream past up to 16 rows (new tokens times the query heads of a key head), which are the M of the MMAs whether or
+// not all of them are in use: S = Q K^T, weights, O += P V, fp32 sums, maximum and sum per row kept while the keys pass.  Bound by HBM: the
+// MMAs take a quarter of the time that the keys take from memory.
+// A CTA is four warps and works off a slot of the work list; two of them share an SM.  Of a block of 64 keys a warp takes 16, which it
+// copies for itself (cp.async, a ring of its own, a row of the block table per key, so that pages may have any size and end anywhere):
+// the loop over the keys has no barrier, and the copies run ahead over the ends of tiles.  At the end of a tile, or of the slot, the
+// warps' results are joined in shared memory in the order of the warps.  Tiles whose keys are spread over several slots leave partial
+// results (numerator, maximum, sum) that join_kernel adds up in the order of the slots.
+constexpr int RW_THREADS = 128, RW_WARPS = 4, RW_WARP_KEYS = PG_KEYS / RW_WARPS;
+
+template <int DP> struct RowsShape {
+	static constexpr int UNITS = DP / 8;                            // 16-byte units of a row
+	static constexpr int HALF = RW_WARP_KEYS * DP * 2;              // bytes of a warp's keys, and of its values
+	static constexpr int STAGES = DP == 64 ? 5 : 3;
+	static constexpr int RING = RW_WARPS * STAGES * 2 * HALF;
+	static constexpr int JOIN = RW_WARPS * PG_ROWS * (DP / 2 < 64 ? DP / 2 : 64) * 4;
+	static constexpr int SMEM = RING + JOIN;
+};
+
+struct Walk {                          // a place in the units of a slot
+	int entry, kv, block, blocks;
+	int64_t left;
+	PgEntry e;
+};
+__device__ __forceinline__ PgEntry read_entry(const PgEntry *p) {
+	const int4 a = __ldg(reinterpret_cast<const int4 *>(p)), b = __ldg(reinterpret_cast<const int4 *>(p) + 1);
+	return PgEntry{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
+__device__ __forceinline__ bool step(Walk &w, const PgEntry *entries, int kv_heads) {          // false: no unit is left
+	if (--w.left <= 0) return false;
+	if (++w.block == w.e.blocks) {
+		w.block = 0;
+		if (++w.kv == kv_heads) {
+			w.kv = 0;
+			w.e = read_entry(entries + ++w.entry);
+		}
+	}
+	return true;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(const paged_attention_t p, const PgWork work) {
+	using S = RowsShape<DP>;
+	extern __shared__ __align__(128) unsigned char rw_smem[];
+	__shared__ float s_m[RW_WARPS][PG_ROWS], s_l[RW_WARPS][PG_ROWS];
+	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
+	const PgList list = work.list[0];
+	const PgEntry *entries = work.entries[0];
+	const int slot = blockIdx.x;
+	const int64_t u0 = slot * list.per;
+	if (u0 >= list.total) return;
+	const PgStart start = work.starts[0][slot];
+	Walk at = {start.entry, start.kv, start.block, 0, min(list.per, list.total - u0), read_entry(entries + start.entry)};
+	Walk ahead = at;                                     // what is copied next
+	const int group = p.heads / p.kv_heads;
+	const uint32_t ring = smem_u32(rw_smem) + warp * S::STAGES * 2 * S::HALF;
+	float *s_join = reinterpret_cast<float *>(rw_smem + S::RING);
+	const float to_base2 = p.scale * PG_LOG2E;
+	const int units = p.dim / 8;
+	int bad = 0;
+
+	// The lower half of the warp looks after the 16 keys, the upper half after their values: the page of key (lane & 15) of the unit.
+	const T *cache = reinterpret_cast<const T *>(lane < 16 ? p.k_cache : p.v_cache);
+	const int64_t page_step = lane < 16 ? p.k_page : p.v_page, kv_step = lane < 16 ? p.k_kv : p.v_kv;
+	bool more = true;
+	int next_id = -1, next_row = 0;                      // page (-1: no key there) and row in it
+	auto look_up = [&]() {
+		const int key = ahead.block * PG_KEYS + warp * RW_WARP_KEYS + (lane & 15);
+		next_id = -1;
+		next_row = 0;
+		if (key < ahead.e.seen) {
+			const int c = key / p.page;
+			next_row = key - c * p.page;
+			next_id = c < p.table_width ? __ldg(p.table + (int64_t)ahead.e.request * p.table_ld + c) : -2;
+		}
+	};
+	auto copy = [&](int stage) {
+		const bool there = next_id >= 0 && next_id < p.pages;
+		if (next_id != -1 && !there) bad = PAGED_BAD_INDEX;
+		const T *src = there ? cache + next_id * page_step + ahead.kv * kv_step + (int64_t)next_row * p.dim : cache;
+		const unsigned long long mine = reinterpret_cast<unsigned long long>(src) | (there ? 1ull : 0ull);          // (addresses are even)
+		const uint32_t dst = ring + stage * 2 * S::HALF;
+#pragma unroll
+		for (int i = 0; i < 2 * RW_WARP_KEYS * S::UNITS / 32; ++i) {
+			const int x = lane + 32 * i, row = x / S::UNITS, unit = x % S::UNITS;          // rows 16 .. are values
+			const unsigned long long theirs = __shfl_sync(0xffffffffu, mine, row);
+			const bool real = (theirs & 1ull) && unit < units;
+			cp_async16_or_zero(dst + row * DP * 2 + ((unit ^ (row & 7)) << 4), reinterpret_cast<const unsigned char *>(theirs & ~1ull) + (real ? unit * 16 : 0), real ? 16 : 0);
+		}
+		more = step(ahead, entries, p.kv_heads);
+		if (more) look_up();
+	};
+	look_up();
+#pragma unroll
+	for (int s = 0; s < S::STAGES; ++s) {
+		if (more) copy(s);
+		cp_async_commit();
+	}
+
+	uint32_t q[DP / 16][4];
+	float o[DP / 8][4], mx[2], sum[2];
+	int seen[2];                                          // keys that rows gid and gid + 8 see
+	int least = 0;                                        // ... and that the row with the fewest of them sees
+	bool fresh = true;
+	int first_block = at.block;
+	for (int stage = 0;;) {
+		if (fresh) {                                      // a new tile or key head: its queries
+			fresh = false;
+			first_block = at.block;
+			const int count = min(PG_ROWS, at.e.fresh * group - at.e.tile * PG_ROWS);
+			least = at.e.len - at.e.fresh + at.e.tile * PG_ROWS / group + 1;
+#pragma unroll
+			for (int i = 0; i < 2; ++i) {
+				const int row = gid + 8 * i, token = (at.e.tile * PG_ROWS + row) / group, head = at.kv * group + (at.e.tile * PG_ROWS + row) - token * group;
+				seen[i] = row < count ? at.e.len - at.e.fresh + token + 1 : 0;
+				const T *src = reinterpret_cast<const T *>(p.q) + (int64_t)(at.e.row + token) * p.q_row + (int64_t)head * p.q_head;
+#pragma unroll
+				for (int k = 0; k < DP / 16; ++k) {
+					const int d = 16 * k + 2 * tig;
+					q[k][i] = row < count && d < p.dim ? *reinterpret_cast<const uint32_t *>(src + d) : 0u;
+					q[k][2 + i] = row < count && d + 8 < p.dim ? *reinterpret_cast<const uint32_t *>(src + d + 8) : 0u;
+				}
+				mx[i] = -INFINITY;
+				sum[i] = 0.f;
+			}
+#pragma unroll
+			for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+				for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+		}
+		cp_async_wait<S::STAGES - 1>();
+		__syncwarp();
+		const uint32_t sk = ring + (uint32_t)stage * 2 * S::HALF, sv = sk + S::HALF;
+		const int key0 = at.block * PG_KEYS + warp * RW_WARP_KEYS;
+		{
+			float s[2][4] = {};
+			const int kr = (lane >> 4) * 8 + (lane & 7), ku = (lane >> 3) & 1;
+#pragma unroll
+			for (int k = 0; k < DP / 16; ++k) {
+				uint32_t b[4];
+				ldsm4(b, sk + kr * DP * 2 + (((2 * k + ku) ^ (kr & 7)) << 4));
+				mma16<T>(s[0], q[k], b[0], b[1]);
+				mma16<T>(s[1], q[k], b[2], b[3]);
+			}
+			const bool edge = key0 + RW_WARP_KEYS > least;
+			float top[2];
+#pragma unroll
+			for (int i = 0; i < 2; ++i) {
+#pragma unroll
+				for (int t = 0; t < 2; ++t)
+#pragma unroll
+					for (int j = 0; j < 2; ++j) {
+						float &x = s[t][2 * i + j];
+						x *= to_base2;
+						if (edge && key0 + 8 * t + 2 * tig + j >= seen[i]) x = -INFINITY;
+					}
+				float m = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+				m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+				m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+				top[i] = fmaxf(m, mx[i]);
+			}
+			if (__any_sync(0xffffffffu, top[0] > mx[0] || top[1] > mx[1])) {
+#pragma unroll
+				for (int i = 0; i < 2; ++i) {
+					const float keep = mx[i] == -INFINITY ? 0.f : ex2(mx[i] - top[i]);
+					mx[i] = top[i];
+					sum[i] *= keep;
+#pragma unroll
+					for (int t = 0; t < DP / 8; ++t) {
+						o[t][2 * i] *= keep;
+						o[t][2 * i + 1] *= keep;
+					}
+				}
+			}
+			uint32_t w[4];
+#pragma unroll
+			for (int i = 0; i < 2; ++i) {
+				const float ref = mx[i] == -INFINITY ? 0.f : mx[i];
+				const float a = ex2(s[0][2 * i] - ref), b = ex2(s[0][2 * i + 1] - ref), c = ex2(s[1][2 * i] - ref), d = ex2(s[1][2 * i + 1] - ref);
+				sum[i] += (a + b) + (c + d);
+				// weights in the type of the values, at most 1: what the MMA multiplies; their sum is taken before the rounding
+				w[i] = pack2<T>(a, b);
+				w[2 + i] = pack2<T>(c, d);
+			}
+			const int vr = ((lane >> 3) & 1) * 8 + (lane & 7), vu = lane >> 4;
+#pragma unroll
+			for (int t = 0; t < DP / 16; ++t) {
+				uint32_t b[4];
+				ldsm4_t(b, sv + vr * DP * 2 + (((2 * t + vu) ^ (vr & 7)) << 4));
+				mma16<T>(o[2 * t], w, b[0], b[1]);
+				mma16<T>(o[2 * t + 1], w, b[2], b[3]);
+			}
+		}
+		__syncwarp();
+		if (more) copy(stage);
+		cp_async_commit();
+		stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+
+		const bool tile_ends = at.block + 1 == at.e.blocks;
+		const Walk here = at;
+		const bool go_on = step(at, entries, p.kv_heads);
+		if (!tile_ends && go_on) continue;
+		// ---- the warps' shares ----
+		fresh = true;
+		const bool whole = first_block == 0 && tile_ends;
+#pragma unroll
+		for (int i = 0; i < 2; ++i) {
+			sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+			sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+			if (tig == 0) {
+				s_m[warp][gid + 8 * i] = mx[i];
+				s_l[warp][gid + 8 * i] = sum[i];
+			}
+		}
+		constexpr int W = DP / 2 < 64 ? DP / 2 : 64;          // columns that are joined at a time
+		const int count = min(PG_ROWS, here.e.fresh * group - here.e.tile * PG_ROWS);
+		float *part = reinterpret_cast<float *>(p.scratch) + (int64_t)(2 * slot + (first_block == 0)) * PG_ROWS * (DP + 2);
+#pragma unroll
+		for (int c0 = 0; c0 < DP; c0 += W) {
+#pragma unroll
+			for (int t = c0 / 8; t < (c0 + W) / 8; ++t)
+#pragma unroll
+				for (int i = 0; i < 2; ++i)
+					*reinterpret_cast<float2 *>(s_join + (warp * PG_ROWS + gid + 8 * i) * W + 8 * t - c0 + 2 * tig) = make_float2(o[t][2 * i], o[t][2 * i + 1]);
+			__syncthreads();
+			for (int x = tid; x < count * (W / 4); x += RW_THREADS) {
+				const int row = x / (W / 4), col = x % (W / 4) * 4;
+				float m = -INFINITY;
+#pragma unroll
+				for (int v = 0; v < RW_WARPS; ++v) m = fmaxf(m, s_m[v][row]);
+				float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+				float l = 0.f;
+#pragma unroll
+				for (int v = 0; v < RW_WARPS; ++v) {
+					const float f = s_m[v][row] == -INFINITY ? 0.f : ex2(s_m[v][row] - m);
+					const float4 y = *reinterpret_cast<const float4 *>(s_join + (v * PG_ROWS + row) * W + col);
+					l = fmaf(s_l[v][row], f, l);
+					a = make_float4(fmaf(y.x, f, a.x), fmaf(y.y, f, a.y), fmaf(y.z, f, a.z), fmaf(y.w, f, a.w));
+				}
+				if (whole) {
+					const int token = (here.e.tile * PG_ROWS + row) / group, head = here.kv * group + here.e.tile * PG_ROWS + row - token * group;
+					const float f = here.e.len - here.e.fresh + token < 0 ? 0.f : 1.f / l;
+					if (c0 + col < p.dim)
+						*reinterpret_cast<uint2 *>(reinterpret_cast<T *>(p.out) + ((int64_t)(here.e.row + token) * p.heads + head) * p.dim + c0 + col) = make_uint2(pack2<T>(a.x * f, a.y * f), pack2<T>(a.z * f, a.w * f));
+				} else {
+					__stcg(reinterpret_cast<float4 *>(part + row * DP + c0 + col), a);
+					if (c0 == 0 && col == 0) __stcg(reinterpret_cast<float2 *>(part + PG_ROWS * DP + 2 * row), make_float2(m, l));
+				}
+			}
+			__syncthreads();
+		}
+		if (!go_on) break;
+	}
+	if (bad) atomicOr(p.status, bad);
+}
+
+// CTA c joins the tile whose keys begin in slot c and end in a later one.
+template <typename T, int DP>
+__global__ void __launch_bounds__(RW_THREADS) join_kernel(const paged_attention_t p, const PgWork work) {
+	const PgList list = work.list[0];
+	const int slot = blockIdx.x, tid = threadIdx.x, group = p.heads / p.kv_heads;
+	const int64_t u1 = (slot + 1) * list.per;
+	if (u1 >= list.total) return;
+	const PgStart s = work.starts[0][slot + 1];
+	if (s.block == 0 || s.block > list.per) return;
+	const PgEntry e = read_entry(work.entries[0] + s.entry);
+	const int more = (int)((e.blocks - s.block + list.per - 1) / list.per);          // further slots
+	const int count = min(PG_ROWS, e.fresh * group - e.tile * PG_ROWS);
+	const float *scratch = reinterpret_cast<const float *>(p.scratch);
+	auto part = [&](int i) { return scratch + (int64_t)(i == 0 ? 2 * slot + 1 : 2 * (slot + i)) * PG_ROWS * (DP + 2); };
+	for (int x = tid; x < count * (DP / 4); x += RW_THREADS) {
+		const int row = x / (DP / 4), col = x % (DP / 4) * 4;
+		float m = -INFINITY, l = 0.f;
+		float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+		for (int i = 0; i <= more; ++i) {
+			const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(i) + PG_ROWS * DP + 2 * row));
+			const float4 y = __ldcg(reinterpret_cast<const float4 *>(part(i) + row * DP + col));
+			const float top = fmaxf(m, ml.x), keep = m == -INFINITY ? 0.f : ex2(m - top), f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+			m = top;
+			l = fmaf(l, keep, ml.y * f);
+			a = make_float4(fmaf(a.x, keep, y.x * f), fmaf(a.y, keep, y.y * f), fmaf(a.z, keep, y.z * f), fmaf(a.w, keep, y.w * f));
+		}
+		const int token = (e.tile * PG_ROWS + row) / group, head = s.kv * group + e.tile * PG_ROWS + row - token * group;
+		const float f = e.len - e.fresh + token < 0 ? 0.f : 1.f / l;
+		if (col < p.dim)
+			*reinterpret_cast<uint2 *>(reinterpret_cast<T *>(p.out) + ((int64_t)(e.row + token) * p.heads + head) * p.dim + col) = make_uint2(pack2<T>(a.x * f, a.y * f), pack2<T>(a.z * f, a.w * f));
+	}
+}
+
+int rows_dp(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+template <typename T, int DP>
+int rows_launch(const paged_attention_t &p, const PgWork &work, cudaStream_t stream) {
+	constexpr int smem = RowsShape<DP>::SMEM;
+	static_assert(smem + 1536 <= (DP <= 128 ? 114 : 228) * 1024, "shared memory of an SM, 1 KB of it reserved per CTA");
+	if (int rc = cuda_status(cudaFuncSetAttribute(rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return rc;
+	rows_kernel<T, DP><<<PG_SLOTS, RW_THREADS, smem, stream>>>(p, work);
+	if (int rc = cuda_status(cudaGetLastError())) return rc;
+	join_kernel<T, DP><<<PG_SLOTS, RW_THREADS, 0, stream>>>(p, work);
+	return cuda_status(cudaGetLastError());
+}
+template <typename T>
+int rows_launch_dim(const paged_attention_t &p, const PgWork &work, cudaStream_t stream) {
+	switch (rows_dp(p.dim)) {
+		case 64: return rows_launch<T, 64>(p, work, stream);
+		case 128: return rows_launch<T, 128>(p, work, stream);
+		default: return rows_launch<T, 256>(p, work, stream);
+	}
+}
+
 }   // namespace
+
+int64_t pg_rows_scratch(const paged_attention_t &p) { return (int64_t)2 * PG_SLOTS * PG_ROWS * (rows_dp(p.dim) + 2) * 4; }
+
+int pg_rows_launch(const paged_attention_t &p, int dtype, cudaStream_t stream) {
+	const PgWork work = pg_work(const_cast<int32_t *>(p.work), p.requests, p.rows, p.heads, p.kv_heads);
+	return dtype == PG_BF16 ? rows_launch_dim<bf16>(p, work, stream) : rows_launch_dim<__half>(p, work, stream);
+}
 
 int pg_attend_simple(const paged_attention_t &p, int dtype, cudaStream_t stream) {
 	const unsigned ctas = (unsigned)(((int64_t)p.rows * p.heads + 3) / 4);
