@@ -75,7 +75,7 @@ inline __host__ __device__ PgWork pg_work(int32_t *base, int requests, int rows,
 }
 // Whether the tensor-core kernel serves these sizes; which requests it then takes (more rows than PG_ROWS) is decided on the device.
 inline bool pg_tiles_serve(int dtype, int dim, int page, int max_fresh, int heads, int kv_heads) {
-	return false;
+	return dtype != PG_F32 && dim <= 128 && dim % 8 == 0 && (page == 8 || page == 16 || page == 32 || page == 64 || page % PG_TILE_KEYS == 0) && (int64_t)max_fresh * (heads / kv_heads) > PG_ROWS;
 }
 
 // cp.async of 16 bytes; `bytes` 0 writes zeros and reads nothing
@@ -118,6 +118,8 @@ int pg_plan_launch(const paged_plan_t &p, int dtype, cudaStream_t stream);
 int pg_append_launch(const paged_append_t &p, int dtype, cudaStream_t stream);
 int64_t pg_rows_scratch(const paged_attention_t &p);
 int pg_rows_launch(const paged_attention_t &p, int dtype, cudaStream_t stream);          // fp16, bf16
+int64_t pg_tiles_scratch(const paged_attention_t &p);
+int pg_tiles_launch(const paged_attention_t &p, int dtype, char *scratch, cudaStream_t stream);
 int pg_attend_simple(const paged_attention_t &p, int dtype, cudaStream_t stream);
 
 }   // namespace gptq

@@ -15,7 +15,9 @@ bool known(int dtype) { return dtype == PG_BF16 || dtype == PG_F32 || dtype == P
 int size_of(int dtype) { return dtype == PG_F32 ? 4 : 2; }
 bool heads_ok(int heads, int kv_heads) { return kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && heads <= 65535; }
 // heads and pages start on 16 bytes
-bool steps_ok(int64_t a, int64_t b, int dtype) { return a >= 0 && b >= 0 && a * size_of(dtype) % 16 == 0 && b * size_of(dtype) % 16 == 0; }
+bool steps_ok(int64_t a, int64_t b, int dtype) { return a * size_of(dtype) % 16 == 0 && b * size_of(dtype) % 16 == 0; }
+
+bool tiles(const paged_attention_t &p, int dtype) { return p.pages > 0 && pg_tiles_serve(dtype, p.dim, p.page, p.max_fresh, p.heads, p.kv_heads); }
 
 }   // namespace
 
@@ -50,7 +52,8 @@ int paged_append(const paged_append_t *p, int dtype, void *stream) {
 
 int64_t paged_attention_scratch(const paged_attention_t *p, int dtype) {
 	if (!p || !known(dtype) || p->dim < 1 || p->dim > PAGED_MAX_DIM) return -1;
-	return dtype == PG_F32 ? 16 : pg_rows_scratch(*p);
+	if (!heads_ok(p->heads, p->kv_heads) || p->page < 1) return -1;
+	return dtype == PG_F32 ? 16 : pg_rows_scratch(*p) + (tiles(*p, dtype) ? pg_tiles_scratch(*p) : 0);
 }
 
 int paged_attention(const paged_attention_t *p, int dtype, void *stream) {
@@ -60,11 +63,19 @@ int paged_attention(const paged_attention_t *p, int dtype, void *stream) {
 	if (p->dim < 1 || p->dim > PAGED_MAX_DIM || p->dim % 8) return GPTQ_ERR_SHAPE;
 	if (p->requests == 0 || p->rows == 0) return GPTQ_OK;
 	if (!p->q || !p->k_cache || !p->v_cache || !p->table || !p->row_start || !p->lens || !p->work || !p->out) return GPTQ_ERR_INVALID;
+	// pages, and key heads within them, are places of their own
+	const int64_t least = (int64_t)p->page * p->dim;
+	for (int64_t s : {p->k_page, p->v_page})
+		if (p->pages > 1 && s < least) return GPTQ_ERR_INVALID;
+	for (int64_t s : {p->k_kv, p->v_kv})
+		if (p->kv_heads > 1 && s < least) return GPTQ_ERR_INVALID;
 	if (!steps_ok(p->k_page, p->k_kv, dtype) || !steps_ok(p->v_page, p->v_kv, dtype) || !steps_ok(p->q_row, p->q_head, dtype) || !aligned16(p->q) || !aligned16(p->k_cache) || !aligned16(p->v_cache) ||
 		!aligned16(p->out))
 		return GPTQ_ERR_ALIGN;
 	if (dtype == PG_F32) return pg_attend_simple(*p, dtype, (cudaStream_t)stream);
-	if (!p->scratch || !aligned16(p->scratch) || (int64_t)p->scratch_bytes < pg_rows_scratch(*p)) return GPTQ_ERR_WORKSPACE;
+	if (!p->scratch || !aligned16(p->scratch) || (int64_t)p->scratch_bytes < paged_attention_scratch(p, dtype)) return GPTQ_ERR_WORKSPACE;
+	if (tiles(*p, dtype))
+		if (int rc = pg_tiles_launch(*p, dtype, (char *)p->scratch + pg_rows_scratch(*p), (cudaStream_t)stream)) return rc;
 	return pg_rows_launch(*p, dtype, (cudaStream_t)stream);
 }
 

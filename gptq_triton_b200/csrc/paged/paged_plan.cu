@@ -84,6 +84,7 @@ __device__ __forceinline__ Lengths lengths_of(const paged_plan_t &p, int r, int 
 // What the attention sees of a request is at most what its table can name.
 __device__ __forceinline__ int length_seen(const paged_plan_t &p, const Lengths &l) { return (int)min((int64_t)l.past + l.fresh, min((int64_t)p.table_width * p.page, (int64_t)PL_LIMIT)); }
 
+constexpr int PL_JOIN = 6;
 constexpr int PL_KEEP = 4096;          // units before an entry that are kept in shared memory for the search
 
 // The work list of one kernel.  s_tiles [R + 1]: tiles of the requests before; s_first: PL_KEEP ints.
@@ -116,8 +117,41 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 		units = add_to(units, total, PL_LIMIT);
 	}
 	__syncthreads();
-	const int64_t total = (int64_t)units * p.kv_heads, per = max((total + slots - 1) / slots, (int64_t)(kind ? 2 : 2));
-	if (tid == 0) w.list[kind] = PgList{E, 0, per, total};
+	const int64_t total = (int64_t)units * p.kv_heads, per = max((total + slots - 1) / slots, (int64_t)2);
+	int whole = 0;
+	if (kind) {
+		// Whole tiles, the longest first, dealt out to the slots forwards and backwards in turn, unless the longest slot would then work
+		// PL_JOIN blocks longer than equal ranges take: that is what partial results and the kernel that joins them cost.
+		__shared__ int s_most, s_span, s_hist[PL_THREADS];
+		if (tid == 0) s_most = s_span = 0;
+		s_hist[tid] = 0;
+		__syncthreads();
+		if (E <= PL_KEEP) {
+			for (int e = tid; e < E; e += PL_THREADS) atomicMax(&s_most, w.entries[1][e].blocks);
+			__syncthreads();
+			auto bucket = [&](int n) { return PL_THREADS - 1 - (int)((int64_t)n * (PL_THREADS - 1) / s_most); };
+			for (int e = tid; e < E; e += PL_THREADS) atomicAdd(&s_hist[bucket(w.entries[1][e].blocks)], 1);
+			__syncthreads();
+			int a = s_hist[tid], b = 0, ta, tb;
+			scan2(a, b, PL_LIMIT, PL_LIMIT, ta, tb, s_scan);
+			s_hist[tid] = a;
+			__syncthreads();
+			// (tiles of one length are in no particular order: which slot takes one changes no result)
+			for (int e = tid; e < E; e += PL_THREADS) w.order[atomicAdd(&s_hist[bucket(w.entries[1][e].blocks)], 1)] = e;
+		} else {
+			for (int e = tid; e < E; e += PL_THREADS) w.order[e] = e;
+		}
+		__syncthreads();
+		const int64_t items = (int64_t)E * p.kv_heads;
+		if (tid < slots) {
+			int64_t sum = 0;
+			for (int64_t turn = 0, i = tid; i < items; ++turn, i = turn & 1 ? (turn + 1) * slots - 1 - tid : turn * slots + tid) sum += w.entries[1][w.order[i / p.kv_heads]].blocks;
+			atomicMax(&s_span, (int)min(sum, (int64_t)PL_LIMIT));
+		}
+		__syncthreads();
+		whole = s_span <= per + PL_JOIN;
+	}
+	if (tid == 0) w.list[kind] = PgList{E, whole, per, total};
 	for (int c = tid; c <= slots; c += PL_THREADS) {
 		const int64_t u = c * per;
 		PgStart s = {-1, 0, 0, 0};
@@ -258,7 +292,7 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, 
 }   // namespace
 
 int pg_plan_launch(const paged_plan_t &p, int dtype, cudaStream_t stream) {
-	const int tiles = pg_tiles_serve(dtype, p.dim, p.page, p.max_fresh, p.heads, p.kv_heads);
+	const int tiles = p.pages > 0 && pg_tiles_serve(dtype, p.dim, p.page, p.max_fresh, p.heads, p.kv_heads);
 	const size_t smem = (size_t)(4 * (p.requests + 1) + PL_KEEP) * sizeof(int);
 	static_assert((4 * (PAGED_MAX_REQUESTS + 1) + PL_KEEP) * sizeof(int) + 4096 <= 227 * 1024, "shared memory");
 	if (smem > 48 * 1024 - 4096)
