@@ -146,12 +146,12 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 	using S = TileShape<DP>;
 	constexpr bool F16 = sizeof(T) == 2 && !std::is_same<T, bf16>::value;
 	extern __shared__ unsigned char tl_raw[];
-	__shared__ uint64_t s_bars[2 * S::RING + 9];
+	__shared__ uint64_t s_bars[2 * S::RING + 11];
 	__shared__ uint32_t s_tmem;
 	__shared__ int s_stop;
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = p.heads / p.kv_heads;
 	const uint32_t sq = (smem_u32(tl_raw) + 1023u) & ~1023u, ring = sq + 2 * S::BLOCK;
-	const uint32_t bars = smem_u32(s_bars), bar_full = bars, bar_free = bars + 8 * S::RING, bar_q = bars + 16 * S::RING, bar_s = bar_q + 16, bar_p = bar_q + 32, bar_o = bar_q + 48, bar_end = bar_q + 64;
+	const uint32_t bars = smem_u32(s_bars), bar_full = bars, bar_free = bars + 8 * S::RING, bar_q = bars + 16 * S::RING, bar_s = bar_q + 16, bar_p = bar_q + 32, bar_o = bar_q + 48, bar_none = bar_q + 64, bar_end = bar_q + 80;
 	volatile int *stop = &s_stop;
 	Items it(work, p.kv_heads, blockIdx.x);
 	bool have = it.next();
@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 			mbar_init(bar_s + 8 * i, 1);
 			mbar_init(bar_p + 8 * i, TL_SIDE);
 			mbar_init(bar_o + 8 * i, 1);
+			mbar_init(bar_none + 8 * i, 1);
 		}
 		mbar_init(bar_end, 1);
 		s_stop = 0;
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 			for (int s = 0; s < 2 && ok; ++s) {
 				if (!wait(bar_q + 8 * s, nq)) break;
 				if (it.j0 < ends[s]) qk(s, n);
-				else commit(bar_o + 8 * s);              // nothing for this side: it waits for this before it goes on to the next tile
+				else commit(bar_none + 8 * s);
 			}
 			if (!ok) break;
 			commit(bar_free + 8 * (n % S::RING));
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 		const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + side * TL_KEYS + lane_base, to = tmem + S::O_AT + side * DP + lane_base;
 		const float scale2 = p.scale * PG_LOG2E;
 		constexpr float LIFT = F16 ? 7.f : 0.f;            // fp16 weights up to 2^15: small ones stay above its subnormal range
-		uint32_t ns = 0, no = 0;
+		uint32_t ns = 0, no = 0, nn = 0;
 		bool ok = true;
 		auto wait = [&](uint32_t bar, uint32_t parity) {
 			ok = ok && wait_fast(bar, parity & 1, stop);
@@ -402,7 +403,9 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 			// the next tile's queries go first: its scores are computed while this one's results are stored
 			const PgEntry e = it.e;
 			const int kv = it.kv, j0 = it.j0, j1 = it.j1, my_token = token, my_head = head, my_sees = sees;
-			if (j0 >= end && !wait(bar_o + 8 * side, no++)) break;          // a side without blocks must not run ahead of the MMA warp
+			// A side without blocks in this tile must not run ahead of the MMA warp: a wait tells a phase from its neighbours only.  (Not bar_o:
+			// the MMA warp may come to this while the results of the tile before still wait to be read.)
+			if (j0 >= end && !wait(bar_none + 8 * side, nn++)) break;
 			have = it.next();
 			if (have) queries();
 			float a, b;

@@ -222,5 +222,15 @@ def test_chunks(dtype, past, new, heads, kv_heads, dim, page):
 	check_attention(Step(past, new, heads, kv_heads, dim, page, dtype, seed=new[0]))
 
 
+@pytest.mark.parametrize('seed', range(4))
+@pytest.mark.parametrize('heads,kv_heads,dim', [(16, 16, 64), (12, 4, 128)])
+def test_many_tiles(seed, heads, kv_heads, dim):
+	"""Several tiles per processor one after the other, full ones, ones with rows on one side only, short and long ones."""
+	import random
+	rng = random.Random(seed)
+	new = [rng.choice([1, 7, 20, 90, 128, 140, 256, 257, 300, 511]) for _ in range(24)]
+	check_attention(Step([rng.choice([0, 0, 5, 130]) for _ in new], new, heads, kv_heads, dim, 32, 'bf16' if seed % 2 else 'fp16', seed=seed, pad=1))
+
+
 def test_requests_that_all_wait():
 	check_attention(Step([5, 0], [0, 0], 4, 2, 64, 16, 'fp16', pad=4))
