@@ -23,7 +23,8 @@ namespace {
 
 constexpr int TL_SIDE = 128, TL_KEYS = PG_TILE_KEYS;
 constexpr int TL_CHUNK = 128 * 128;                      // bytes of 128 rows of 64 columns
-constexpr int TL_THREADS = 320, TL_TMA = 8, TL_MMA = 9;
+constexpr int TL_THREADS = 384, TL_TMA = 8, TL_MMA = 9;          // (warps 10 and 11 complete the third warpgroup)
+constexpr int TL_REGS_SOFTMAX = 208, TL_REGS_OTHER = 88;          // of 168 at launch: 2 * 208 + 88 = 3 * 168
 constexpr uint32_t TL_SPIN = 1u << 24;                  // polls of a bounded wait
 
 template <int DP> struct TileShape {
@@ -39,7 +40,7 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *tmap, int 
 				 "r"(c1), "r"(c2), "r"(c3), "r"(bar)
 				 : "memory");
 }
-static __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int *abort_flag) { return !*abort_flag && mbar_wait_bounded(bar, parity, TL_SPIN); }
+__device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int *abort_flag) { return !*abort_flag && mbar_wait_bounded(bar, parity, TL_SPIN); }
 __device__ __forceinline__ bool wait_fast(uint32_t bar, uint32_t parity, volatile int *abort_flag) { return mbar_try_wait(bar, parity) || wait_slow(bar, parity, abort_flag); }
 // registers loaded by tcgen05.ld may be used only behind the wait: tie them to it
 template <int N>
@@ -78,13 +79,13 @@ struct Items {
 	const PgEntry *entries;
 	const int *order;
 	int slot, slots, kv_heads, whole, entry;
-	int64_t left, turn, count;
+	int left, turn, count;             // (a slot's share and the number of tiles are far below 2^31: the plan's sums stop at 2^30 per key head)
 	__device__ Items(const PgWork &w, int kvh, int s) : entries(w.entries[1]), order(w.order), slot(s), slots(PG_TILE_SLOTS), kv_heads(kvh) {
 		const PgList l = w.list[1];
 		whole = l.whole;
 		turn = 0;
-		count = (int64_t)l.entries * kvh;
-		left = min(l.per, l.total - (int64_t)s * l.per);
+		count = (int)min((int64_t)l.entries * kvh, (int64_t)1 << 30);
+		left = (int)max(min(min(l.per, (int64_t)1 << 30), l.total - (int64_t)s * l.per), (int64_t)0);
 		kv = j1 = 0;
 		entry = 0;
 		if (!whole && left > 0) {
@@ -101,10 +102,10 @@ struct Items {
 	}
 	__device__ bool next() {
 		if (whole) {                     // sorted by length, dealt out forwards and backwards in turn
-			const int64_t i = turn & 1 ? (turn + 1) * slots - 1 - slot : turn * slots + slot;
+			const int i = turn & 1 ? (turn + 1) * slots - 1 - slot : turn * slots + slot;
 			++turn;
 			if (i >= count) return false;
-			kv = (int)(i % kv_heads);
+			kv = i % kv_heads;
 			e = read(__ldg(order + i / kv_heads));
 			j0 = 0;
 			j1 = e.blocks;
@@ -119,7 +120,7 @@ struct Items {
 			}
 		}
 		j0 = j1;
-		j1 = (int)min((int64_t)e.blocks, j0 + left);
+		j1 = e.blocks - j0 < left ? e.blocks : j0 + left;
 		left -= j1 - j0;
 		return true;
 	}
@@ -146,12 +147,12 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 	using S = TileShape<DP>;
 	constexpr bool F16 = sizeof(T) == 2 && !std::is_same<T, bf16>::value;
 	extern __shared__ unsigned char tl_raw[];
-	__shared__ uint64_t s_bars[2 * S::RING + 11];
+	__shared__ uint64_t s_bars[2 * S::RING + 13];
 	__shared__ uint32_t s_tmem;
 	__shared__ int s_stop;
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = p.heads / p.kv_heads;
 	const uint32_t sq = (smem_u32(tl_raw) + 1023u) & ~1023u, ring = sq + 2 * S::BLOCK;
-	const uint32_t bars = smem_u32(s_bars), bar_full = bars, bar_free = bars + 8 * S::RING, bar_q = bars + 16 * S::RING, bar_s = bar_q + 16, bar_p = bar_q + 32, bar_o = bar_q + 48, bar_none = bar_q + 64, bar_end = bar_q + 80;
+	const uint32_t bars = smem_u32(s_bars), bar_full = bars, bar_free = bars + 8 * S::RING, bar_q = bars + 16 * S::RING, bar_s = bar_q + 16, bar_p = bar_q + 32, bar_o = bar_q + 48, bar_none = bar_q + 64, bar_p2 = bar_q + 80, bar_end = bar_q + 96;
 	volatile int *stop = &s_stop;
 	Items it(work, p.kv_heads, blockIdx.x);
 	bool have = it.next();
@@ -165,6 +166,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 			mbar_init(bar_q + 8 * i, TL_SIDE);
 			mbar_init(bar_s + 8 * i, 1);
 			mbar_init(bar_p + 8 * i, TL_SIDE);
+			mbar_init(bar_p2 + 8 * i, TL_SIDE);
 			mbar_init(bar_o + 8 * i, 1);
 			mbar_init(bar_none + 8 * i, 1);
 		}
@@ -185,6 +187,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 		atomicOr(p.status, 3);
 	};
 
+	if (warp >= 8) {
+		asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TL_REGS_OTHER));
 	if (warp == TL_TMA) {
 		// lane: page `mine / CHUNKS` of a block, columns 64 (mine % CHUNKS) ..
 		const int per_block = p.page < TL_KEYS ? TL_KEYS / p.page : 1, loads = per_block * S::CHUNKS, box = min(p.page, TL_KEYS);
@@ -226,7 +230,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 		for (int i = max(0, n - S::RING); i < n; ++i) mbar_wait_bounded(bar_full + 8 * (i % S::RING), (i / S::RING) & 1, TL_SPIN);
 		if (bad) atomicOr(p.status, bad);
 		__syncwarp();
-	} else if (warp == TL_MMA) {
+	}
+	if (warp == TL_MMA) {
 		constexpr uint32_t base = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(TL_SIDE >> 4) << 24);          // D fp32, M = 128
 		constexpr uint32_t id_qk = base | ((uint32_t)(TL_KEYS >> 3) << 17), id_pv = base | (1u << 16) | ((uint32_t)(DP >> 3) << 17);      // values: N contiguous
 		int n = 0;                                         // blocks of the ring consumed
@@ -251,11 +256,11 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 			}
 			__syncwarp();
 		};
-		auto pv = [&](int s, int i, bool first) {
+		auto pv = [&](int s, int i, int half, bool first) {          // 64 of the 128 keys
 			if (lane == 0) {
 				const uint64_t vd = desc_values(ring + (i % S::RING) * S::BLOCK);
 #pragma unroll
-				for (int k = 0; k < TL_KEYS / 16; ++k) umma_f16_ts(tmem + S::O_AT + s * DP, tmem + s * TL_KEYS + 8 * k, vd + 128 * k, id_pv, first && k == 0 ? 0u : 1u);
+				for (int k = half * (TL_KEYS / 32); k < (half + 1) * (TL_KEYS / 32); ++k) umma_f16_ts(tmem + S::O_AT + s * DP, tmem + s * TL_KEYS + 8 * k, vd + 128 * k, id_pv, first && k == 0 ? 0u : 1u);
 			}
 			__syncwarp();
 		};
@@ -289,7 +294,10 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 				const bool again = j + 1 < it.j1;
 				if (again && !full(n + 2)) break;
 				for (int s = 0; s < 2 && ok; ++s) {
-					if (j < ends[s] && wait(bar_p + 8 * s, np[s]++)) pv(s, n + 1, j == it.j0);
+					if (j < ends[s]) {
+						if (wait(bar_p + 8 * s, np[s])) pv(s, n + 1, 0, j == it.j0);
+						if (wait(bar_p2 + 8 * s, np[s]++)) pv(s, n + 1, 1, false);
+					}
 					if (ok && j + 1 < ends[s]) qk(s, n + 2);
 					if (ok && j + 1 == ends[s]) commit(bar_o + 8 * s);
 				}
@@ -301,7 +309,9 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 		commit(bar_end);                                 // every MMA has completed before tensor memory goes back
 		mbar_wait_bounded(bar_end, 0, TL_SPIN);
 		__syncwarp();
+	}
 	} else {
+		asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TL_REGS_SOFTMAX));
 		const int side = warp >> 2, rl = (warp & 3) * 32 + lane, row = side * TL_SIDE + rl;
 		const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + side * TL_KEYS + lane_base, to = tmem + S::O_AT + side * DP + lane_base;
 		const float scale2 = p.scale * PG_LOG2E;
@@ -394,10 +404,10 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 						w[k] = pack2<T>(a, b);
 					}
 					tmem_st32(ts + 32 * h, w);
+					tmem_st_wait();
+					tc_fence_before();
+					mbar_arrive((h ? bar_p2 : bar_p) + 8 * side);
 				}
-				tmem_st_wait();
-				tc_fence_before();
-				mbar_arrive(bar_p + 8 * side);
 			}
 			if (!ok) break;
 			// the next tile's queries go first: its scores are computed while this one's results are stored
