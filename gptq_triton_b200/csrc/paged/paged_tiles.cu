@@ -52,6 +52,13 @@ __device__ __forceinline__ void tmem_settle(float (&v)[N]) {
 #pragma unroll
 	for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
 }
+// One lane of the warp, known to the compiler as one: operands of the instructions behind `lane == 0` are taken for different ones in
+// every lane, and eight MMAs then took 450 cycles to issue.
+__device__ __forceinline__ bool elect() {
+	uint32_t r;
+	asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+	return r != 0;
+}
 // Values as the B operand: their columns are its N and lie one behind the other; chunks of 64 columns TL_CHUNK apart, a chunk holds
 // rows of 128 bytes (a key each) in groups of 8, 1024 bytes apart; 128-byte swizzle.
 __device__ __forceinline__ uint64_t desc_values(uint32_t addr) {
@@ -239,6 +246,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 	} else if (warp == TL_MMA) {
 		constexpr uint32_t base = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(TL_SIDE >> 4) << 24);          // D fp32, M = 128
 		constexpr uint32_t id_qk = base | ((uint32_t)(TL_KEYS >> 3) << 17), id_pv = base | (1u << 16) | ((uint32_t)(DP >> 3) << 17);      // values: N contiguous
+		const bool one = elect();
 		int n = 0;                                         // blocks of the ring consumed
 		uint32_t nq = 0, np[2] = {0, 0};
 		bool ok = true;
@@ -253,7 +261,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 		};
 		auto full = [&](int i) { return wait(bar_full + 8 * (i % S::RING), i / S::RING); };
 		auto qk = [&](int s, int i) {
-			if (lane == 0) {
+			if (one) {
 				const uint64_t qd = smem_desc_sw128(sq + s * S::BLOCK), kd = smem_desc_sw128(ring + (i % S::RING) * S::BLOCK);
 #pragma unroll
 				for (int k = 0; k < DP / 16; ++k) umma_f16(tmem + s * TL_KEYS, qd + (k >> 2) * (TL_CHUNK / 16) + 2 * (k & 3), kd + (k >> 2) * (TL_CHUNK / 16) + 2 * (k & 3), id_qk, k ? 1u : 0u);
@@ -262,7 +270,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 			__syncwarp();
 		};
 		auto pv = [&](int s, int i, int half, bool first) {          // 64 of the 128 keys
-			if (lane == 0) {
+			if (one) {
 				const uint64_t vd = desc_values(ring + (i % S::RING) * S::BLOCK);
 #pragma unroll
 				for (int k = half * (TL_KEYS / 32); k < (half + 1) * (TL_KEYS / 32); ++k) umma_f16_ts(tmem + S::O_AT + s * DP, tmem + s * TL_KEYS + (k >> 2) * 64 + (k & 3) * 8, vd + 128 * k, id_pv, first && k == 0 ? 0u : 1u);
@@ -270,7 +278,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 			__syncwarp();
 		};
 		auto commit = [&](uint32_t bar) {
-			if (lane == 0) umma_commit(bar);
+			if (one) umma_commit(bar);
 			__syncwarp();
 		};
 		for (; have && ok; have = it.next(), ++nq) {
