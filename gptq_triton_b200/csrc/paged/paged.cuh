@@ -1,6 +1,10 @@
 // Shared pieces of the paged-cache library: argument blocks, element access, the layout of the attention's work lists.
 #pragma once
 
+#include <atomic>
+#include <type_traits>
+#include <utility>
+
 #include <cuda_bf16.h>
 
 #include "../common.cuh"
@@ -45,6 +49,21 @@ struct PgEntry {
 	int row, fresh, len, seen;          // first row and new tokens of the request, its tokens, those that the tile's last row sees
 };
 struct PgStart { int entry, kv, block, pad; };                 // entry -1: nothing to do
+
+// Everything that an earlier kernel wrote is read through L2: under programmatic dependent launch a line may have come to L1 before.
+__device__ __forceinline__ PgList read_list(const PgList *p) {
+	const int2 a = __ldcg(reinterpret_cast<const int2 *>(p));
+	const long long b = __ldcg(reinterpret_cast<const long long *>(p) + 1), c = __ldcg(reinterpret_cast<const long long *>(p) + 2);
+	return PgList{a.x, a.y, b, c};
+}
+__device__ __forceinline__ PgStart read_start(const PgStart *p) {
+	const int4 a = __ldcg(reinterpret_cast<const int4 *>(p));
+	return PgStart{a.x, a.y, a.z, a.w};
+}
+__device__ __forceinline__ PgEntry read_entry(const PgEntry *p) {
+	const int4 a = __ldcg(reinterpret_cast<const int4 *>(p)), b = __ldcg(reinterpret_cast<const int4 *>(p) + 1);
+	return PgEntry{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
 
 struct PgWork {
 	PgList *list;                       // [2]
@@ -114,10 +133,31 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 	asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
+// Launch with programmatic stream serialisation: every kernel of this library touches nothing that an earlier one wrote, and writes
+// nothing, before its pdl_wait(), and triggers its successor behind it.  (The kernel for few rows is the exception, see there.)
+int pg_smem_opt_in(const void *kernel);
+template <typename... KArgs, typename... Args>
+int pg_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args &&...args) {
+	if (smem > 16 * 1024)          // (static shared memory comes on top)
+		if (int rc = pg_smem_opt_in(reinterpret_cast<const void *>(kernel))) return rc;
+	cudaLaunchConfig_t cfg = {};
+	cfg.gridDim = grid;
+	cfg.blockDim = dim3(threads);
+	cfg.dynamicSmemBytes = smem;
+	cfg.stream = stream;
+	cudaLaunchAttribute attr;
+	attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	attr.val.programmaticStreamSerializationAllowed = 1;
+	cfg.attrs = &attr;
+	cfg.numAttrs = 1;
+	return cuda_status(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
+
 int pg_plan_launch(const paged_plan_t &p, int dtype, cudaStream_t stream);
 int pg_append_launch(const paged_append_t &p, int dtype, cudaStream_t stream);
 int64_t pg_rows_scratch(const paged_attention_t &p);
-int pg_rows_launch(const paged_attention_t &p, int dtype, cudaStream_t stream);          // fp16, bf16
+int pg_rows_launch(const paged_attention_t &p, int dtype, bool beside, cudaStream_t stream);          // fp16, bf16; beside: the tile kernel runs
+int pg_join_launch(const paged_attention_t &p, int dtype, char *tile_scratch, cudaStream_t stream);          // of both kernels
 int64_t pg_tiles_scratch(const paged_attention_t &p);
 int pg_tiles_launch(const paged_attention_t &p, int dtype, char *scratch, cudaStream_t stream);
 int pg_attend_simple(const paged_attention_t &p, int dtype, cudaStream_t stream);

@@ -1,10 +1,28 @@
 // C ABI of the paged-cache library: checks of arguments and the choice of kernels.
-#include <new>
-
 #include "paged.cuh"
 
 namespace gptq {
 thread_local int g_last_cuda_error = 0;
+
+// All the shared memory that a kernel may have, asked for once per kernel and device.
+int pg_smem_opt_in(const void *kernel) {
+	static std::atomic<const void *> kernels[32];
+	static std::atomic<unsigned long long> devices[32];
+	int dev = 0, i = 0;
+	if (int rc = cuda_status(cudaGetDevice(&dev))) return rc;
+	for (; i < 32; ++i) {
+		const void *seen = kernels[i].load();
+		if (!seen && kernels[i].compare_exchange_strong(seen, kernel)) seen = kernel;
+		if (seen == kernel) break;
+	}
+	const bool kept = i < 32 && dev < 64;
+	if (kept && devices[i].load() >> dev & 1) return GPTQ_OK;
+	cudaFuncAttributes attr;
+	if (int rc = cuda_status(cudaFuncGetAttributes(&attr, kernel))) return rc;
+	if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)attr.sharedSizeBytes))) return rc;
+	if (kept) devices[i].fetch_or(1ull << dev);
+	return GPTQ_OK;
+}
 }
 
 using namespace gptq;
@@ -74,9 +92,12 @@ int paged_attention(const paged_attention_t *p, int dtype, void *stream) {
 		return GPTQ_ERR_ALIGN;
 	if (dtype == PG_F32) return pg_attend_simple(*p, dtype, (cudaStream_t)stream);
 	if (!p->scratch || !aligned16(p->scratch) || (int64_t)p->scratch_bytes < paged_attention_scratch(p, dtype)) return GPTQ_ERR_WORKSPACE;
-	if (tiles(*p, dtype))
-		if (int rc = pg_tiles_launch(*p, dtype, (char *)p->scratch + pg_rows_scratch(*p), (cudaStream_t)stream)) return rc;
-	return pg_rows_launch(*p, dtype, (cudaStream_t)stream);
+	const bool both = tiles(*p, dtype);
+	char *tile_scratch = both ? (char *)p->scratch + pg_rows_scratch(*p) : nullptr;
+	if (both)
+		if (int rc = pg_tiles_launch(*p, dtype, tile_scratch, (cudaStream_t)stream)) return rc;
+	if (int rc = pg_rows_launch(*p, dtype, both, (cudaStream_t)stream)) return rc;
+	return pg_join_launch(*p, dtype, tile_scratch, (cudaStream_t)stream);
 }
 
 }   // extern "C"

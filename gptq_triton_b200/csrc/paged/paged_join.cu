@@ -1,0 +1,77 @@
+// Joins the partial results of tiles whose keys are spread over several slots of an attention kernel: numerators, maxima (base 2) and sums
+// of a row, in the order of the slots.
+//   m = max m_i,  l = sum l_i 2^(m_i - m),  out = (sum a_i 2^(m_i - m)) / l
+// A tile that is spread begins in exactly one slot: CTA c looks whether one begins in slot c and ends in a later one.
+#include "paged.cuh"
+
+namespace gptq {
+
+namespace {
+
+constexpr int JN_THREADS = 128, JN_ROWS = 16;            // rows of a tile that a CTA joins
+
+template <typename T> __device__ __forceinline__ void store_four(T *dst, float4 v) { *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w)); }
+template <> __device__ __forceinline__ void store_four<float>(float *dst, float4 v) { *reinterpret_cast<float4 *>(dst) = v; }
+
+// kind 0: tiles of PG_ROWS rows, 1: of PG_TILE rows; DP: columns of a partial result
+template <typename T, int DP>
+__device__ void join(const paged_attention_t &p, const PgWork &work, int kind, int slot, int row0, const float *scratch) {
+	const PgList list = read_list(work.list + kind);
+	const int group = p.heads / p.kv_heads, tile_rows = kind ? PG_TILE : PG_ROWS;
+	if (list.whole || (slot + 1) * list.per >= list.total) return;
+	const PgStart s = read_start(work.starts[kind] + slot + 1);
+	if (s.block == 0 || s.block > list.per) return;
+	const PgEntry e = read_entry(work.entries[kind] + s.entry);
+	const int more = (int)((e.blocks - s.block + list.per - 1) / list.per);          // further slots
+	auto part = [&](int i) { return scratch + (int64_t)(i == 0 ? 2 * slot + 1 : 2 * (slot + i)) * tile_rows * (DP + 2); };
+	for (int x = threadIdx.x; x < JN_ROWS * (DP / 4); x += JN_THREADS) {
+		const int row = row0 + x / (DP / 4), col = x % (DP / 4) * 4;
+		const int64_t at = (int64_t)e.tile * tile_rows + row;
+		if (at >= (int64_t)e.fresh * group || col >= p.dim) continue;
+		float m = -INFINITY, l = 0.f;
+		float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+		for (int i = 0; i <= more; ++i) {
+			const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(i) + (int64_t)tile_rows * DP) + row);
+			const float4 y = __ldcg(reinterpret_cast<const float4 *>(part(i) + (int64_t)row * DP + col));
+			const float top = fmaxf(m, ml.x), keep = m == -INFINITY ? 0.f : ex2(m - top), f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+			m = top;
+			l = fmaf(l, keep, ml.y * f);
+			a = make_float4(fmaf(a.x, keep, y.x * f), fmaf(a.y, keep, y.y * f), fmaf(a.z, keep, y.z * f), fmaf(a.w, keep, y.w * f));
+		}
+		const int token = (int)(at / group), head = (int)(at - (int64_t)token * group);
+		const bool blind = e.len - e.fresh + token < 0;          // a row that sees nothing
+		const float f = 1.f / l;
+		store_four<T>(reinterpret_cast<T *>(p.out) + ((int64_t)(e.row + token) * p.heads + s.kv * group + head) * p.dim + col,
+					  blind ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(a.x * f, a.y * f, a.z * f, a.w * f));
+	}
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(JN_THREADS) join_kernel(const paged_attention_t p, const PgWork work, const float *tile_scratch) {
+	pdl_wait();
+	pdl_trigger();
+	if (blockIdx.x < PG_SLOTS) {
+		join<T, DP>(p, work, 0, blockIdx.x, 0, reinterpret_cast<const float *>(p.scratch));
+	} else if (DP <= 128) {
+		const int x = blockIdx.x - PG_SLOTS;
+		join<T, DP>(p, work, 1, x % PG_TILE_SLOTS, x / PG_TILE_SLOTS * JN_ROWS, tile_scratch);
+	}
+}
+
+template <typename T>
+int launch(const paged_attention_t &p, const float *tile_scratch, cudaStream_t stream) {
+	const PgWork work = pg_work(const_cast<int32_t *>(p.work), p.requests, p.rows, p.heads, p.kv_heads);
+	const dim3 grid(PG_SLOTS + (tile_scratch ? PG_TILE_SLOTS * (PG_TILE / JN_ROWS) : 0));
+	if (p.dim <= 64) return pg_launch(join_kernel<T, 64>, grid, JN_THREADS, 0, stream, p, work, tile_scratch);
+	if (p.dim <= 128) return pg_launch(join_kernel<T, 128>, grid, JN_THREADS, 0, stream, p, work, tile_scratch);
+	return pg_launch(join_kernel<T, 256>, grid, JN_THREADS, 0, stream, p, work, tile_scratch);
+}
+
+}   // namespace
+
+int pg_join_launch(const paged_attention_t &p, int dtype, char *tile_scratch, cudaStream_t stream) {
+	const float *t = reinterpret_cast<const float *>(tile_scratch);
+	return dtype == PG_BF16 ? launch<bf16>(p, t, stream) : dtype == PG_F16 ? launch<__half>(p, t, stream) : launch<float>(p, t, stream);
+}
+
+}   // namespace gptq

@@ -68,8 +68,8 @@ struct Lengths { int past, fresh, old, full; };
 
 __device__ __forceinline__ Lengths lengths_of(const paged_plan_t &p, int r, int &bad) {
 	Lengths l;
-	l.past = __ldg(p.past + r);
-	l.fresh = __ldg(p.fresh + r);
+	l.past = __ldcg(p.past + r);
+	l.fresh = __ldcg(p.fresh + r);
 	if (l.past < 0 || l.past > PL_LIMIT || l.fresh < 0 || l.fresh > PL_LIMIT / 2) {
 		bad |= PAGED_BAD_INDEX;
 		l.past = min(max(l.past, 0), PL_LIMIT);
@@ -185,6 +185,8 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, 
 	__shared__ int s_scan[64];
 	int *s_start = pl_smem, *s_off = pl_smem + p.requests + 1;
 	const int tid = threadIdx.x, R = p.requests;
+	pdl_wait();
+	pdl_trigger();
 	int bad = 0, rows = 0, taken = 0;
 	for (int base = 0; base < R; base += PL_THREADS) {
 		const int r = base + tid;
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, 
 	if (tid == 0) s_start[R] = min(rows, p.rows);
 	if (rows > p.rows) bad |= PAGED_NO_ROOM;
 	__syncthreads();
-	const int head = p.pool ? __ldg(p.head) : 0, used = s_start[R];
+	const int head = p.pool ? __ldcg(p.head) : 0, used = s_start[R];
 	if (p.pool && (head < 0 || head > p.pool_size || taken > p.pool_size - head)) bad |= head < 0 || head > p.pool_size ? PAGED_BAD_INDEX : PAGED_NO_ROOM;
 
 	// the page that entry c of request r names; -1: none
@@ -214,9 +216,9 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, 
 		int id;
 		if (p.pool && c >= old) {
 			const long long at = (long long)head + s_off[r] + (c - old);
-			id = at >= 0 && at < p.pool_size ? __ldg(p.pool + at) : -1;
+			id = at >= 0 && at < p.pool_size ? __ldcg(p.pool + at) : -1;
 		} else {
-			id = c < p.table_width ? p.table[(int64_t)r * p.table_ld + c] : -1;
+			id = c < p.table_width ? __ldcg(p.table + (int64_t)r * p.table_ld + c) : -1;
 		}
 		return id;
 	};
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, 
 			int64_t slot = -1;
 			if (m < used) {
 				const int r = find(s_start, R, m);
-				const int past = min(max(__ldg(p.past + r), 0), PL_LIMIT);
+				const int past = min(max(__ldcg(p.past + r), 0), PL_LIMIT);
 				pos = past + m - s_start[r];
 				const int c = pos / p.page;
 				const int id = page_of(r, c, (past + p.page - 1) / p.page);
@@ -295,11 +297,8 @@ int pg_plan_launch(const paged_plan_t &p, int dtype, cudaStream_t stream) {
 	const int tiles = p.pages > 0 && pg_tiles_serve(dtype, p.dim, p.page, p.max_fresh, p.heads, p.kv_heads);
 	const size_t smem = (size_t)(4 * (p.requests + 1) + PL_KEEP) * sizeof(int);
 	static_assert((4 * (PAGED_MAX_REQUESTS + 1) + PL_KEEP) * sizeof(int) + 4096 <= 227 * 1024, "shared memory");
-	if (smem > 48 * 1024 - 4096)
-		if (int rc = cuda_status(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))) return rc;
 	const int fill = (int)((p.rows + (int64_t)PL_THREADS - 1) / PL_THREADS), ctas = 1 + (fill < 1 ? 1 : fill > 295 ? 295 : fill);
-	plan_kernel<<<ctas, PL_THREADS, smem, stream>>>(p, tiles);
-	return cuda_status(cudaGetLastError());
+	return pg_launch(plan_kernel, dim3(ctas), PL_THREADS, smem, stream, p, tiles);
 }
 
 }   // namespace gptq

@@ -9,6 +9,8 @@ namespace {
 // maximum and sum.
 template <typename T>
 __global__ void __launch_bounds__(128) simple_kernel(const paged_attention_t p) {
+	pdl_wait();
+	pdl_trigger();
 	const int lane = threadIdx.x & 31;
 	const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
 	const int m = (int)(at / p.heads), h = (int)(at % p.heads), kvh = h / (p.heads / p.kv_heads);
@@ -79,10 +81,6 @@ struct Walk {                          // a place in the units of a slot
 	int64_t left;
 	PgEntry e;
 };
-__device__ __forceinline__ PgEntry read_entry(const PgEntry *p) {
-	const int4 a = __ldg(reinterpret_cast<const int4 *>(p)), b = __ldg(reinterpret_cast<const int4 *>(p) + 1);
-	return PgEntry{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-}
 __device__ __forceinline__ bool step(Walk &w, const PgEntry *entries, int kv_heads) {          // false: no unit is left
 	if (--w.left <= 0) return false;
 	if (++w.block == w.e.blocks) {
@@ -96,17 +94,24 @@ __device__ __forceinline__ bool step(Walk &w, const PgEntry *entries, int kv_hea
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(const paged_attention_t p, const PgWork work) {
+__global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(const paged_attention_t p, const PgWork work, int beside) {
 	using S = RowsShape<DP>;
 	extern __shared__ __align__(128) unsigned char rw_smem[];
 	__shared__ float s_m[RW_WARPS][PG_ROWS], s_l[RW_WARPS][PG_ROWS];
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
-	const PgList list = work.list[0];
+	// Beside the tile kernel this one needs nothing of it and runs as soon as SMs are free: what came before the tile kernel is complete
+	// when that triggers, and the wait is at the end, so that whoever waits for this kernel waits for both.
+	if (!beside) pdl_wait();
+	pdl_trigger();
+	const PgList list = read_list(work.list);
 	const PgEntry *entries = work.entries[0];
 	const int slot = blockIdx.x;
 	const int64_t u0 = slot * list.per;
-	if (u0 >= list.total) return;
-	const PgStart start = work.starts[0][slot];
+	if (u0 >= list.total) {
+		if (beside) pdl_wait();
+		return;
+	}
+	const PgStart start = read_start(work.starts[0] + slot);
 	Walk at = {start.entry, start.kv, start.block, 0, min(list.per, list.total - u0), read_entry(entries + start.entry)};
 	Walk ahead = at;                                     // what is copied next
 	const int group = p.heads / p.kv_heads;
@@ -128,7 +133,7 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 		if (key < ahead.e.seen) {
 			const int c = key / p.page;
 			next_row = key - c * p.page;
-			next_id = c < p.table_width ? __ldg(p.table + (int64_t)ahead.e.request * p.table_ld + c) : -2;
+			next_id = c < p.table_width ? __ldcg(p.table + (int64_t)ahead.e.request * p.table_ld + c) : -2;
 		}
 	};
 	auto copy = [&](int stage) {
@@ -174,8 +179,8 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 #pragma unroll
 				for (int k = 0; k < DP / 16; ++k) {
 					const int d = 16 * k + 2 * tig;
-					q[k][i] = row < count && d < p.dim ? *reinterpret_cast<const uint32_t *>(src + d) : 0u;
-					q[k][2 + i] = row < count && d + 8 < p.dim ? *reinterpret_cast<const uint32_t *>(src + d + 8) : 0u;
+					q[k][i] = row < count && d < p.dim ? __ldcg(reinterpret_cast<const uint32_t *>(src + d)) : 0u;
+					q[k][2 + i] = row < count && d + 8 < p.dim ? __ldcg(reinterpret_cast<const uint32_t *>(src + d + 8)) : 0u;
 				}
 				mx[i] = -INFINITY;
 				sum[i] = 0.f;
@@ -309,59 +314,23 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 		if (!go_on) break;
 	}
 	if (bad) atomicOr(p.status, bad);
-}
-
-// CTA c joins the tile whose keys begin in slot c and end in a later one.
-template <typename T, int DP>
-__global__ void __launch_bounds__(RW_THREADS) join_kernel(const paged_attention_t p, const PgWork work) {
-	const PgList list = work.list[0];
-	const int slot = blockIdx.x, tid = threadIdx.x, group = p.heads / p.kv_heads;
-	const int64_t u1 = (slot + 1) * list.per;
-	if (u1 >= list.total) return;
-	const PgStart s = work.starts[0][slot + 1];
-	if (s.block == 0 || s.block > list.per) return;
-	const PgEntry e = read_entry(work.entries[0] + s.entry);
-	const int more = (int)((e.blocks - s.block + list.per - 1) / list.per);          // further slots
-	const int count = min(PG_ROWS, e.fresh * group - e.tile * PG_ROWS);
-	const float *scratch = reinterpret_cast<const float *>(p.scratch);
-	auto part = [&](int i) { return scratch + (int64_t)(i == 0 ? 2 * slot + 1 : 2 * (slot + i)) * PG_ROWS * (DP + 2); };
-	for (int x = tid; x < count * (DP / 4); x += RW_THREADS) {
-		const int row = x / (DP / 4), col = x % (DP / 4) * 4;
-		float m = -INFINITY, l = 0.f;
-		float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-		for (int i = 0; i <= more; ++i) {
-			const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(i) + PG_ROWS * DP + 2 * row));
-			const float4 y = __ldcg(reinterpret_cast<const float4 *>(part(i) + row * DP + col));
-			const float top = fmaxf(m, ml.x), keep = m == -INFINITY ? 0.f : ex2(m - top), f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-			m = top;
-			l = fmaf(l, keep, ml.y * f);
-			a = make_float4(fmaf(a.x, keep, y.x * f), fmaf(a.y, keep, y.y * f), fmaf(a.z, keep, y.z * f), fmaf(a.w, keep, y.w * f));
-		}
-		const int token = (e.tile * PG_ROWS + row) / group, head = s.kv * group + e.tile * PG_ROWS + row - token * group;
-		const float f = e.len - e.fresh + token < 0 ? 0.f : 1.f / l;
-		if (col < p.dim)
-			*reinterpret_cast<uint2 *>(reinterpret_cast<T *>(p.out) + ((int64_t)(e.row + token) * p.heads + head) * p.dim + col) = make_uint2(pack2<T>(a.x * f, a.y * f), pack2<T>(a.z * f, a.w * f));
-	}
+	if (beside) pdl_wait();
 }
 
 int rows_dp(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 template <typename T, int DP>
-int rows_launch(const paged_attention_t &p, const PgWork &work, cudaStream_t stream) {
+int rows_launch(const paged_attention_t &p, const PgWork &work, bool beside, cudaStream_t stream) {
 	constexpr int smem = RowsShape<DP>::SMEM;
 	static_assert(smem + 1536 <= (DP <= 128 ? 114 : 228) * 1024, "shared memory of an SM, 1 KB of it reserved per CTA");
-	if (int rc = cuda_status(cudaFuncSetAttribute(rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return rc;
-	rows_kernel<T, DP><<<PG_SLOTS, RW_THREADS, smem, stream>>>(p, work);
-	if (int rc = cuda_status(cudaGetLastError())) return rc;
-	join_kernel<T, DP><<<PG_SLOTS, RW_THREADS, 0, stream>>>(p, work);
-	return cuda_status(cudaGetLastError());
+	return pg_launch(rows_kernel<T, DP>, dim3(PG_SLOTS), RW_THREADS, smem, stream, p, work, (int)beside);
 }
 template <typename T>
-int rows_launch_dim(const paged_attention_t &p, const PgWork &work, cudaStream_t stream) {
+int rows_launch_dim(const paged_attention_t &p, const PgWork &work, bool beside, cudaStream_t stream) {
 	switch (rows_dp(p.dim)) {
-		case 64: return rows_launch<T, 64>(p, work, stream);
-		case 128: return rows_launch<T, 128>(p, work, stream);
-		default: return rows_launch<T, 256>(p, work, stream);
+		case 64: return rows_launch<T, 64>(p, work, beside, stream);
+		case 128: return rows_launch<T, 128>(p, work, beside, stream);
+		default: return rows_launch<T, 256>(p, work, beside, stream);
 	}
 }
 
@@ -369,17 +338,15 @@ int rows_launch_dim(const paged_attention_t &p, const PgWork &work, cudaStream_t
 
 int64_t pg_rows_scratch(const paged_attention_t &p) { return (int64_t)2 * PG_SLOTS * PG_ROWS * (rows_dp(p.dim) + 2) * 4; }
 
-int pg_rows_launch(const paged_attention_t &p, int dtype, cudaStream_t stream) {
+int pg_rows_launch(const paged_attention_t &p, int dtype, bool beside, cudaStream_t stream) {
 	const PgWork work = pg_work(const_cast<int32_t *>(p.work), p.requests, p.rows, p.heads, p.kv_heads);
-	return dtype == PG_BF16 ? rows_launch_dim<bf16>(p, work, stream) : rows_launch_dim<__half>(p, work, stream);
+	return dtype == PG_BF16 ? rows_launch_dim<bf16>(p, work, beside, stream) : rows_launch_dim<__half>(p, work, beside, stream);
 }
 
 int pg_attend_simple(const paged_attention_t &p, int dtype, cudaStream_t stream) {
 	const unsigned ctas = (unsigned)(((int64_t)p.rows * p.heads + 3) / 4);
-	if (dtype == PG_F32) simple_kernel<float><<<ctas, 128, 0, stream>>>(p);
-	else if (dtype == PG_BF16) simple_kernel<bf16><<<ctas, 128, 0, stream>>>(p);
-	else simple_kernel<__half><<<ctas, 128, 0, stream>>>(p);
-	return cuda_status(cudaGetLastError());
+	if (dtype == PG_F32) return pg_launch(simple_kernel<float>, dim3(ctas), 128, 0, stream, p);
+	return dtype == PG_BF16 ? pg_launch(simple_kernel<bf16>, dim3(ctas), 128, 0, stream, p) : pg_launch(simple_kernel<__half>, dim3(ctas), 128, 0, stream, p);
 }
 
 }   // namespace gptq
