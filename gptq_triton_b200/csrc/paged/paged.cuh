@@ -32,23 +32,29 @@ template <> struct PgElem<__half> {
 
 // ---- how the attention's work is laid out (paged_plan_t.work) ---------------------------------------------------------------
 // The rows of a request under one key head are its new tokens times the query heads of that key head, token-major.  A tile is a run
-// of them: PG_ROWS rows for the kernel that streams keys past few rows, PG_TILE for the tensor-core kernel; a unit is one tile, one
-// key head and a block of keys (PG_KEYS, PG_TILE_KEYS).  Entries list the tiles, units are counted entry by entry, key head by key head,
-// keys ascending.  Slot c of a kernel works off units [c * per, (c + 1) * per): every slot has as much to do as any other, whatever the
-// lengths, and a tile's keys may be spread over neighbouring slots, whose partial results are then joined.
-constexpr int PG_ROWS = 16, PG_KEYS = 64, PG_SLOTS = 296;
+// of them: PG_ROWS rows for the kernel that streams keys past few rows, PG_TILE for the tensor-core kernel; its keys come in blocks of
+// PG_KEYS, PG_TILE_KEYS.  A job is one tile under one key head.  Entries list the tiles; jobs follow one another entry by entry, key head
+// by key head.  Laid end to end, each as long as its blocks and PG_BEGIN (what a job costs besides: queries, results), they are cut
+// into equal lengths for the slots (warps of one kernel, CTAs of the other): whatever the lengths of the requests, no slot has more to
+// do than another.  A cut inside a job leaves partial results, which are joined; slot c works from starts[c] to starts[c + 1].
+constexpr int PG_ROWS = 16, PG_KEYS = 16, PG_SLOTS = 1184;
 constexpr int PG_TILE = 256, PG_TILE_KEYS = 128, PG_TILE_SLOTS = 148;
+inline __host__ __device__ int pg_begin(int kind) { return kind ? 2 : 1; }
 
 struct PgList {                        // of one of the two kernels; behind it in `work`: starts, entries, order
 	int entries;
-	int whole;                          // slots take whole tiles by `order` instead (tile kernel)
-	int64_t per, total;                 // units of all key heads
+	int whole;                          // slots take whole jobs by `order` instead (tile kernel)
+	int64_t per, total;                 // length of a slot's share, of all jobs
 };
 struct PgEntry {
-	int request, tile, blocks, first;   // blocks of keys that the tile sees; units of the entries before, per key head
+	int request, tile, blocks, first;   // blocks of keys that the tile sees; length of the entries before, per key head
 	int row, fresh, len, seen;          // first row and new tokens of the request, its tokens, those that the tile's last row sees
 };
-struct PgStart { int entry, kv, block, pad; };                 // entry -1: nothing to do
+struct PgStart {                       // entry -1: behind the last job
+	int entry, kv, block, pad;
+	__device__ bool in_job(int e, int k) const { return entry == e && kv == k; }
+	__device__ bool before(int e, int k) const { return entry >= 0 && (entry < e || (entry == e && kv < k)); }          // its job comes before
+};
 
 // Everything that an earlier kernel wrote is read through L2: under programmatic dependent launch a line may have come to L1 before.
 __device__ __forceinline__ PgList read_list(const PgList *p) {

@@ -16,13 +16,28 @@ template <> __device__ __forceinline__ void store_four<float>(float *dst, float4
 // kind 0: tiles of PG_ROWS rows, 1: of PG_TILE rows; DP: columns of a partial result
 template <typename T, int DP>
 __device__ void join(const paged_attention_t &p, const PgWork &work, int kind, int slot, int row0, const float *scratch) {
-	const PgList list = read_list(work.list + kind);
-	const int group = p.heads / p.kv_heads, tile_rows = kind ? PG_TILE : PG_ROWS;
-	if (list.whole || (slot + 1) * list.per >= list.total) return;
-	const PgStart s = read_start(work.starts[kind] + slot + 1);
-	if (s.block == 0 || s.block > list.per) return;
+	const int group = p.heads / p.kv_heads, tile_rows = kind ? PG_TILE : PG_ROWS, slots = kind ? PG_TILE_SLOTS : PG_SLOTS;
+	if (read_list(work.list + kind).whole) return;
+	const PgStart *starts = work.starts[kind];
+	const PgStart s = read_start(starts + slot + 1), before = read_start(starts + slot);
+	if (s.entry < 0 || s.block == 0 || (before.in_job(s.entry, s.kv) && before.block > 0)) return;
 	const PgEntry e = read_entry(work.entries[kind] + s.entry);
-	const int more = (int)((e.blocks - s.block + list.per - 1) / list.per);          // further slots
+	if (row0 >= (int64_t)e.fresh * group - (int64_t)e.tile * tile_rows) return;
+	// further slots that begin inside the job
+	int more = 1;
+	for (;; more += 32) {
+		const int c = slot + 1 + more + (threadIdx.x & 31);
+		bool inside = false;
+		if (c <= slots) {
+			const PgStart n = read_start(starts + c);
+			inside = n.in_job(s.entry, s.kv) && n.block > 0;
+		}
+		const unsigned gone = ~__ballot_sync(0xffffffffu, inside);
+		if (gone) {
+			more += __ffs(gone) - 1;
+			break;
+		}
+	}
 	auto part = [&](int i) { return scratch + (int64_t)(i == 0 ? 2 * slot + 1 : 2 * (slot + i)) * tile_rows * (DP + 2); };
 	for (int x = threadIdx.x; x < JN_ROWS * (DP / 4); x += JN_THREADS) {
 		const int row = row0 + x / (DP / 4), col = x % (DP / 4) * 4;
@@ -30,13 +45,31 @@ __device__ void join(const paged_attention_t &p, const PgWork &work, int kind, i
 		if (at >= (int64_t)e.fresh * group || col >= p.dim) continue;
 		float m = -INFINITY, l = 0.f;
 		float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-		for (int i = 0; i <= more; ++i) {
-			const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(i) + (int64_t)tile_rows * DP) + row);
-			const float4 y = __ldcg(reinterpret_cast<const float4 *>(part(i) + (int64_t)row * DP + col));
-			const float top = fmaxf(m, ml.x), keep = m == -INFINITY ? 0.f : ex2(m - top), f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+		constexpr int BATCH = 8;                             // partial results that are asked for at once
+		for (int i0 = 0; i0 <= more; i0 += BATCH) {
+			float2 ml[BATCH];
+			float4 y[BATCH];
+#pragma unroll
+			for (int i = 0; i < BATCH; ++i)
+				if (i0 + i <= more) {
+					ml[i] = __ldcg(reinterpret_cast<const float2 *>(part(i0 + i) + (int64_t)tile_rows * DP) + row);
+					y[i] = __ldcg(reinterpret_cast<const float4 *>(part(i0 + i) + (int64_t)row * DP + col));
+				}
+			float top = m;
+#pragma unroll
+			for (int i = 0; i < BATCH; ++i)
+				if (i0 + i <= more) top = fmaxf(top, ml[i].x);
+			const float keep = m == -INFINITY ? 0.f : ex2(m - top);
 			m = top;
-			l = fmaf(l, keep, ml.y * f);
-			a = make_float4(fmaf(a.x, keep, y.x * f), fmaf(a.y, keep, y.y * f), fmaf(a.z, keep, y.z * f), fmaf(a.w, keep, y.w * f));
+			l *= keep;
+			a = make_float4(a.x * keep, a.y * keep, a.z * keep, a.w * keep);
+#pragma unroll
+			for (int i = 0; i < BATCH; ++i)
+				if (i0 + i <= more) {
+					const float f = ml[i].x == -INFINITY ? 0.f : ex2(ml[i].x - top);
+					l = fmaf(ml[i].y, f, l);
+					a = make_float4(fmaf(y[i].x, f, a.x), fmaf(y[i].y, f, a.y), fmaf(y[i].z, f, a.z), fmaf(y[i].w, f, a.w));
+				}
 		}
 		const int token = (int)(at / group), head = (int)(at - (int64_t)token * group);
 		const bool blind = e.len - e.fresh + token < 0;          // a row that sees nothing

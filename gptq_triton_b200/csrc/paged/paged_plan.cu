@@ -105,7 +105,8 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 			x.len = length_seen(p, lengths_of(p, x.request, bad));
 			const int last = (int)((min((int64_t)x.fresh * group, (int64_t)(x.tile + 1) * tile_rows) - 1) / group);
 			x.seen = min(max(x.len - x.fresh + last + 1, 0), x.len);
-			n = x.blocks = max((x.seen + keys - 1) / keys, 1);
+			x.blocks = max((x.seen + keys - 1) / keys, 1);
+			n = x.blocks + pg_begin(kind);
 		}
 		int total, unused;
 		scan2(n, none, PL_LIMIT, PL_LIMIT, total, unused, s_scan);
@@ -117,7 +118,9 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 		units = add_to(units, total, PL_LIMIT);
 	}
 	__syncthreads();
-	const int64_t total = (int64_t)units * p.kv_heads, per = max((total + slots - 1) / slots, (int64_t)2);
+	// (a share is longer than what a job costs besides its blocks, so that no two slots begin at the same place; shares of less than
+	// four blocks would be mostly partial results)
+	const int64_t total = (int64_t)units * p.kv_heads, per = max((total + slots - 1) / slots, (int64_t)(4 + pg_begin(kind)));
 	int whole = 0;
 	if (kind) {
 		// Whole tiles, the longest first, dealt out to the slots forwards and backwards in turn, unless the longest slot would then work
@@ -145,7 +148,7 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 		const int64_t items = (int64_t)E * p.kv_heads;
 		if (tid < slots) {
 			int64_t sum = 0;
-			for (int64_t turn = 0, i = tid; i < items; ++turn, i = turn & 1 ? (turn + 1) * slots - 1 - tid : turn * slots + tid) sum += w.entries[1][w.order[i / p.kv_heads]].blocks;
+			for (int64_t turn = 0, i = tid; i < items; ++turn, i = turn & 1 ? (turn + 1) * slots - 1 - tid : turn * slots + tid) sum += w.entries[1][w.order[i / p.kv_heads]].blocks + pg_begin(1);
 			atomicMax(&s_span, (int)min(sum, (int64_t)PL_LIMIT));
 		}
 		__syncthreads();
@@ -169,11 +172,11 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 				}
 				e = lo;
 			}
-			const int n = w.entries[kind][e].blocks;
+			const int n = w.entries[kind][e].blocks + pg_begin(kind);
 			const int64_t rest = u - (int64_t)w.entries[kind][e].first * p.kv_heads;
 			s.entry = e;
 			s.kv = (int)(rest / n);
-			s.block = (int)(rest % n);
+			s.block = max((int)(rest % n) - pg_begin(kind), 0);
 		}
 		w.starts[kind][c] = s;
 	}

@@ -60,74 +60,74 @@ __global__ void __launch_bounds__(128) simple_kernel(const paged_attention_t p) 
 // Keys and values stream past up to 16 rows (new tokens times the query heads of a key head), which are the M of the MMAs whether or
 // not all of them are in use: S = Q K^T, weights, O += P V, fp32 sums, maximum and sum per row kept while the keys pass.  Bound by HBM: the
 // MMAs take a quarter of the time that the keys take from memory.
-// A CTA is four warps and works off a slot of the work list; two of them share an SM.  Of a block of 64 keys a warp takes 16, which it
-// copies for itself (cp.async, a ring of its own, a row of the block table per key, so that pages may have any size and end anywhere):
-// the loop over the keys has no barrier, and the copies run ahead over the ends of tiles.  At the end of a tile, or of the slot, the
-// warps' results are joined in shared memory in the order of the warps.  Tiles whose keys are spread over several slots leave partial
-// results (numerator, maximum, sum) that join_kernel adds up in the order of the slots.
-constexpr int RW_THREADS = 128, RW_WARPS = 4, RW_WARP_KEYS = PG_KEYS / RW_WARPS;
+// A warp is a slot of the work list: it copies 16 keys and their values at a time for itself (cp.async, a ring of its own) and meets no
+// other warp, so that there is no barrier, the copies run ahead over the ends of jobs, and many short jobs do not wait for one another.
+// (Four warps that shared a job and joined their results in shared memory took 86 us for 48 requests of 1 to 12 000 keys: some slots
+// had twenty jobs of a block each.)  Cut jobs leave numerator, maximum and sum of the rows in use, which join_kernel adds up.
+constexpr int RW_THREADS = 128, RW_WARPS = 4;
 
 template <int DP> struct RowsShape {
 	static constexpr int UNITS = DP / 8;                            // 16-byte units of a row
-	static constexpr int HALF = RW_WARP_KEYS * DP * 2;              // bytes of a warp's keys, and of its values
-	static constexpr int STAGES = DP == 64 ? 5 : 3;
-	static constexpr int RING = RW_WARPS * STAGES * 2 * HALF;
-	static constexpr int JOIN = RW_WARPS * PG_ROWS * (DP / 2 < 64 ? DP / 2 : 64) * 4;
-	static constexpr int SMEM = RING + JOIN;
+	static constexpr int HALF = PG_KEYS * DP * 2;                   // bytes of the keys of a block, and of their values
+	static constexpr int STAGES = DP == 64 ? 6 : 3;
+	static constexpr int SMEM = RW_WARPS * STAGES * 2 * HALF;
 };
 
-struct Walk {                          // a place in the units of a slot
-	int entry, kv, block, blocks;
-	int64_t left;
+struct Walk {                          // a block of a slot's jobs
+	int entry, kv, block;
 	PgEntry e;
-};
-__device__ __forceinline__ bool step(Walk &w, const PgEntry *entries, int kv_heads) {          // false: no unit is left
-	if (--w.left <= 0) return false;
-	if (++w.block == w.e.blocks) {
-		w.block = 0;
-		if (++w.kv == kv_heads) {
-			w.kv = 0;
-			w.e = read_entry(entries + ++w.entry);
-		}
+	__device__ __forceinline__ bool start(const PgStart &s, const PgStart &end, const PgEntry *entries) {
+		entry = s.entry;
+		kv = s.kv;
+		block = s.block;
+		if (entry < 0 || (end.in_job(entry, kv) && end.block <= block)) return false;
+		e = read_entry(entries + entry);
+		return true;
 	}
-	return true;
-}
+	__device__ __forceinline__ bool step(const PgStart &end, const PgEntry *entries, int entry_count, int kv_heads) {          // false: no block is left
+		if (++block == e.blocks) {
+			block = 0;
+			if (++kv == kv_heads) {
+				kv = 0;
+				if (++entry == entry_count) return false;
+				e = read_entry(entries + entry);
+			}
+		}
+		return !(end.in_job(entry, kv) ? block >= end.block : block == 0 && end.before(entry, kv));
+	}
+};
 
-template <typename T, int DP>
+// EVEN: pages of a multiple of 16 rows, so that the keys of a block lie in one page, one behind the other
+template <typename T, int DP, bool EVEN>
 __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(const paged_attention_t p, const PgWork work, int beside) {
 	using S = RowsShape<DP>;
 	extern __shared__ __align__(128) unsigned char rw_smem[];
-	__shared__ float s_m[RW_WARPS][PG_ROWS], s_l[RW_WARPS][PG_ROWS];
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
+	constexpr float LIFT = std::is_same<T, __half>::value ? 14.f : 0.f;          // fp16 weights up to 2^14: small ones stay above its subnormal range
 	// Beside the tile kernel this one needs nothing of it and runs as soon as SMs are free: what came before the tile kernel is complete
 	// when that triggers, and the wait is at the end, so that whoever waits for this kernel waits for both.
 	if (!beside) pdl_wait();
 	pdl_trigger();
-	const PgList list = read_list(work.list);
+	const int slot = blockIdx.x * RW_WARPS + warp;
 	const PgEntry *entries = work.entries[0];
-	const int slot = blockIdx.x;
-	const int64_t u0 = slot * list.per;
-	if (u0 >= list.total) {
+	const int entry_count = read_list(work.list).entries;
+	const PgStart begin = read_start(work.starts[0] + slot), end = read_start(work.starts[0] + slot + 1);
+	Walk at;
+	if (!at.start(begin, end, entries)) {
 		if (beside) pdl_wait();
 		return;
 	}
-	const PgStart start = read_start(work.starts[0] + slot);
-	Walk at = {start.entry, start.kv, start.block, 0, min(list.per, list.total - u0), read_entry(entries + start.entry)};
 	Walk ahead = at;                                     // what is copied next
 	const int group = p.heads / p.kv_heads;
 	const uint32_t ring = smem_u32(rw_smem) + warp * S::STAGES * 2 * S::HALF;
-	float *s_join = reinterpret_cast<float *>(rw_smem + S::RING);
 	const float to_base2 = p.scale * PG_LOG2E;
 	const int units = p.dim / 8;
 	int bad = 0;
 
-	// The lower half of the warp looks after the 16 keys, the upper half after their values: the page of key (lane & 15) of the unit.
-	const T *cache = reinterpret_cast<const T *>(lane < 16 ? p.k_cache : p.v_cache);
-	const int64_t page_step = lane < 16 ? p.k_page : p.v_page, kv_step = lane < 16 ? p.k_kv : p.v_kv;
 	bool more = true;
-	int next_id = -1, next_row = 0;                      // page (-1: no key there) and row in it
+	int next_id = -1, next_row = 0;                      // page (-1: no key there) and row in it: of the block (EVEN), of key (lane & 15) of it
 	auto look_up = [&]() {
-		const int key = ahead.block * PG_KEYS + warp * RW_WARP_KEYS + (lane & 15);
+		const int key = ahead.block * PG_KEYS + (EVEN ? 0 : lane & 15);
 		next_id = -1;
 		next_row = 0;
 		if (key < ahead.e.seen) {
@@ -139,17 +139,40 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 	auto copy = [&](int stage) {
 		const bool there = next_id >= 0 && next_id < p.pages;
 		if (next_id != -1 && !there) bad = PAGED_BAD_INDEX;
-		const T *src = there ? cache + next_id * page_step + ahead.kv * kv_step + (int64_t)next_row * p.dim : cache;
-		const unsigned long long mine = reinterpret_cast<unsigned long long>(src) | (there ? 1ull : 0ull);          // (addresses are even)
 		const uint32_t dst = ring + stage * 2 * S::HALF;
+		constexpr int LANES = S::UNITS < 32 ? S::UNITS : 32, ROWS = 32 / LANES;      // a row is 16 bytes times LANES lanes
+		const int unit = lane % LANES, sub = lane / LANES;
+		if (EVEN) {
+			const int rows = there ? min(PG_KEYS, ahead.e.seen - ahead.block * PG_KEYS) : 0;
+			const int64_t first = (int64_t)next_row * p.dim + unit * 8;
+			const T *k = reinterpret_cast<const T *>(p.k_cache), *v = reinterpret_cast<const T *>(p.v_cache);
+			if (there) {
+				k += next_id * p.k_page + ahead.kv * p.k_kv + first;
+				v += next_id * p.v_page + ahead.kv * p.v_kv + first;
+			}
 #pragma unroll
-		for (int i = 0; i < 2 * RW_WARP_KEYS * S::UNITS / 32; ++i) {
-			const int x = lane + 32 * i, row = x / S::UNITS, unit = x % S::UNITS;          // rows 16 .. are values
-			const unsigned long long theirs = __shfl_sync(0xffffffffu, mine, row);
-			const bool real = (theirs & 1ull) && unit < units;
-			cp_async16_or_zero(dst + row * DP * 2 + ((unit ^ (row & 7)) << 4), reinterpret_cast<const unsigned char *>(theirs & ~1ull) + (real ? unit * 16 : 0), real ? 16 : 0);
+			for (int r = 0; r < PG_KEYS; r += ROWS) {
+				const int row = r + sub;
+				const bool real = row < rows && unit < units;
+				const uint32_t to = dst + row * DP * 2 + ((unit ^ (row & 7)) << 4);
+				const int64_t from = real ? (int64_t)row * p.dim : 0;
+				cp_async16_or_zero(to, real ? k + from : reinterpret_cast<const T *>(p.k_cache), real ? 16 : 0);
+				cp_async16_or_zero(to + S::HALF, real ? v + from : reinterpret_cast<const T *>(p.v_cache), real ? 16 : 0);
+			}
+		} else {
+			// The lower half of the warp knows where the 16 keys are, the upper half where their values are.
+			const T *cache = reinterpret_cast<const T *>(lane < 16 ? p.k_cache : p.v_cache);
+			const T *src = there ? cache + next_id * (lane < 16 ? p.k_page : p.v_page) + ahead.kv * (lane < 16 ? p.k_kv : p.v_kv) + (int64_t)next_row * p.dim : cache;
+			const unsigned long long mine = reinterpret_cast<unsigned long long>(src) | (there ? 1ull : 0ull);          // (addresses are even)
+#pragma unroll
+			for (int r = 0; r < 2 * PG_KEYS; r += ROWS) {
+				const int row = r + sub;                   // 16 ..: values
+				const unsigned long long theirs = __shfl_sync(0xffffffffu, mine, row);
+				const bool real = (theirs & 1ull) && unit < units;
+				cp_async16_or_zero(dst + row * DP * 2 + ((unit ^ (row & 7)) << 4), reinterpret_cast<const unsigned char *>(theirs & ~1ull) + (real ? unit * 16 : 0), real ? 16 : 0);
+			}
 		}
-		more = step(ahead, entries, p.kv_heads);
+		more = ahead.step(end, entries, entry_count, p.kv_heads);
 		if (more) look_up();
 	};
 	look_up();
@@ -162,14 +185,14 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 	uint32_t q[DP / 16][4];
 	float o[DP / 8][4], mx[2], sum[2];
 	int seen[2];                                          // keys that rows gid and gid + 8 see
-	int least = 0;                                        // ... and that the row with the fewest of them sees
+	int least = 0, count = 0;                             // ... and that the row with the fewest of them sees; rows in use
 	bool fresh = true;
 	int first_block = at.block;
 	for (int stage = 0;;) {
-		if (fresh) {                                      // a new tile or key head: its queries
+		if (fresh) {                                      // a new job: its queries
 			fresh = false;
 			first_block = at.block;
-			const int count = min(PG_ROWS, at.e.fresh * group - at.e.tile * PG_ROWS);
+			count = min(PG_ROWS, at.e.fresh * group - at.e.tile * PG_ROWS);
 			least = at.e.len - at.e.fresh + at.e.tile * PG_ROWS / group + 1;
 #pragma unroll
 			for (int i = 0; i < 2; ++i) {
@@ -193,7 +216,7 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 		cp_async_wait<S::STAGES - 1>();
 		__syncwarp();
 		const uint32_t sk = ring + (uint32_t)stage * 2 * S::HALF, sv = sk + S::HALF;
-		const int key0 = at.block * PG_KEYS + warp * RW_WARP_KEYS;
+		const int key0 = at.block * PG_KEYS;
 		{
 			float s[2][4] = {};
 			const int kr = (lane >> 4) * 8 + (lane & 7), ku = (lane >> 3) & 1;
@@ -204,7 +227,7 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 				mma16<T>(s[0], q[k], b[0], b[1]);
 				mma16<T>(s[1], q[k], b[2], b[3]);
 			}
-			const bool edge = key0 + RW_WARP_KEYS > least;
+			const bool edge = key0 + PG_KEYS > least;
 			float top[2];
 #pragma unroll
 			for (int i = 0; i < 2; ++i) {
@@ -237,10 +260,10 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 			uint32_t w[4];
 #pragma unroll
 			for (int i = 0; i < 2; ++i) {
-				const float ref = mx[i] == -INFINITY ? 0.f : mx[i];
+				const float ref = mx[i] == -INFINITY ? 0.f : mx[i] - LIFT;
 				const float a = ex2(s[0][2 * i] - ref), b = ex2(s[0][2 * i + 1] - ref), c = ex2(s[1][2 * i] - ref), d = ex2(s[1][2 * i + 1] - ref);
 				sum[i] += (a + b) + (c + d);
-				// weights in the type of the values, at most 1: what the MMA multiplies; their sum is taken before the rounding
+				// weights in the type of the values: what the MMA multiplies; their sum is taken before the rounding
 				w[i] = pack2<T>(a, b);
 				w[2 + i] = pack2<T>(c, d);
 			}
@@ -258,58 +281,32 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 		cp_async_commit();
 		stage = stage + 1 == S::STAGES ? 0 : stage + 1;
 
-		const bool tile_ends = at.block + 1 == at.e.blocks;
-		const Walk here = at;
-		const bool go_on = step(at, entries, p.kv_heads);
+		const int blocks = at.e.blocks, last = at.block, entry_row = at.e.row, before = at.e.len - at.e.fresh, tile = at.e.tile, kv = at.kv;
+		const bool tile_ends = last + 1 == blocks, go_on = at.step(end, entries, entry_count, p.kv_heads);
 		if (!tile_ends && go_on) continue;
-		// ---- the warps' shares ----
+		// ---- the job, or this slot's part of it, is done ----
 		fresh = true;
 		const bool whole = first_block == 0 && tile_ends;
-#pragma unroll
-		for (int i = 0; i < 2; ++i) {
-			sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-			sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-			if (tig == 0) {
-				s_m[warp][gid + 8 * i] = mx[i];
-				s_l[warp][gid + 8 * i] = sum[i];
-			}
-		}
-		constexpr int W = DP / 2 < 64 ? DP / 2 : 64;          // columns that are joined at a time
-		const int count = min(PG_ROWS, here.e.fresh * group - here.e.tile * PG_ROWS);
 		float *part = reinterpret_cast<float *>(p.scratch) + (int64_t)(2 * slot + (first_block == 0)) * PG_ROWS * (DP + 2);
 #pragma unroll
-		for (int c0 = 0; c0 < DP; c0 += W) {
+		for (int i = 0; i < 2; ++i) {
+			const int row = gid + 8 * i;
+			sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+			sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+			if (row >= count) continue;
+			if (whole) {
+				const int token = (tile * PG_ROWS + row) / group, head = kv * group + tile * PG_ROWS + row - token * group;
+				const bool blind = before + token < 0;       // a row that sees nothing
+				const float f = 1.f / sum[i];
+				T *dst = reinterpret_cast<T *>(p.out) + ((int64_t)(entry_row + token) * p.heads + head) * p.dim + 2 * tig;
 #pragma unroll
-			for (int t = c0 / 8; t < (c0 + W) / 8; ++t)
+				for (int t = 0; t < DP / 8; ++t)
+					if (8 * t < p.dim) *reinterpret_cast<uint32_t *>(dst + 8 * t) = blind ? 0u : pack2<T>(o[t][2 * i] * f, o[t][2 * i + 1] * f);
+			} else {
+				if (tig == 0) __stcg(reinterpret_cast<float2 *>(part + PG_ROWS * DP) + row, make_float2(mx[i], sum[i]));
 #pragma unroll
-				for (int i = 0; i < 2; ++i)
-					*reinterpret_cast<float2 *>(s_join + (warp * PG_ROWS + gid + 8 * i) * W + 8 * t - c0 + 2 * tig) = make_float2(o[t][2 * i], o[t][2 * i + 1]);
-			__syncthreads();
-			for (int x = tid; x < count * (W / 4); x += RW_THREADS) {
-				const int row = x / (W / 4), col = x % (W / 4) * 4;
-				float m = -INFINITY;
-#pragma unroll
-				for (int v = 0; v < RW_WARPS; ++v) m = fmaxf(m, s_m[v][row]);
-				float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-				float l = 0.f;
-#pragma unroll
-				for (int v = 0; v < RW_WARPS; ++v) {
-					const float f = s_m[v][row] == -INFINITY ? 0.f : ex2(s_m[v][row] - m);
-					const float4 y = *reinterpret_cast<const float4 *>(s_join + (v * PG_ROWS + row) * W + col);
-					l = fmaf(s_l[v][row], f, l);
-					a = make_float4(fmaf(y.x, f, a.x), fmaf(y.y, f, a.y), fmaf(y.z, f, a.z), fmaf(y.w, f, a.w));
-				}
-				if (whole) {
-					const int token = (here.e.tile * PG_ROWS + row) / group, head = here.kv * group + here.e.tile * PG_ROWS + row - token * group;
-					const float f = here.e.len - here.e.fresh + token < 0 ? 0.f : 1.f / l;
-					if (c0 + col < p.dim)
-						*reinterpret_cast<uint2 *>(reinterpret_cast<T *>(p.out) + ((int64_t)(here.e.row + token) * p.heads + head) * p.dim + c0 + col) = make_uint2(pack2<T>(a.x * f, a.y * f), pack2<T>(a.z * f, a.w * f));
-				} else {
-					__stcg(reinterpret_cast<float4 *>(part + row * DP + c0 + col), a);
-					if (c0 == 0 && col == 0) __stcg(reinterpret_cast<float2 *>(part + PG_ROWS * DP + 2 * row), make_float2(m, l));
-				}
+				for (int t = 0; t < DP / 8; ++t) __stcg(reinterpret_cast<float2 *>(part + row * DP + 8 * t + 2 * tig), make_float2(o[t][2 * i], o[t][2 * i + 1]));
 			}
-			__syncthreads();
 		}
 		if (!go_on) break;
 	}
@@ -322,8 +319,10 @@ int rows_dp(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 template <typename T, int DP>
 int rows_launch(const paged_attention_t &p, const PgWork &work, bool beside, cudaStream_t stream) {
 	constexpr int smem = RowsShape<DP>::SMEM;
-	static_assert(smem + 1536 <= (DP <= 128 ? 114 : 228) * 1024, "shared memory of an SM, 1 KB of it reserved per CTA");
-	return pg_launch(rows_kernel<T, DP>, dim3(PG_SLOTS), RW_THREADS, smem, stream, p, work, (int)beside);
+	static_assert(smem + 1024 <= (DP <= 128 ? 114 : 228) * 1024 && smem <= 227 * 1024, "shared memory of an SM, 1 KB of it reserved per CTA");
+	const dim3 grid(PG_SLOTS / RW_WARPS);
+	if (p.page % PG_KEYS == 0) return pg_launch(rows_kernel<T, DP, true>, grid, RW_THREADS, smem, stream, p, work, (int)beside);
+	return pg_launch(rows_kernel<T, DP, false>, grid, RW_THREADS, smem, stream, p, work, (int)beside);
 }
 template <typename T>
 int rows_launch_dim(const paged_attention_t &p, const PgWork &work, bool beside, cudaStream_t stream) {

@@ -83,47 +83,50 @@ struct Items {
 	int kv, j0, j1;                    // key head, blocks of keys
 	const PgEntry *entries;
 	const int *order;
-	int slot, slots, kv_heads, whole, entry;
-	int left, turn, count;             // (a slot's share and the number of tiles are far below 2^31: the plan's sums stop at 2^30 per key head)
-	__device__ Items(const PgWork &w, int kvh, int s) : entries(w.entries[1]), order(w.order), slot(s), slots(PG_TILE_SLOTS), kv_heads(kvh) {
+	PgStart end;                       // where the next slot begins
+	int slot, kv_heads, whole, entry, entry_count, turn;
+	__device__ Items(const PgWork &w, int kvh, int s) : entries(w.entries[1]), order(w.order), slot(s), kv_heads(kvh) {
 		const PgList l = read_list(w.list + 1);
 		whole = l.whole;
+		entry_count = l.entries;
 		turn = 0;
-		count = (int)min((int64_t)l.entries * kvh, (int64_t)1 << 30);
-		left = (int)max(min(min(l.per, (int64_t)1 << 30), l.total - (int64_t)s * l.per), (int64_t)0);
 		kv = j1 = 0;
-		entry = 0;
-		if (!whole && left > 0) {
+		entry = -1;
+		if (!whole) {
 			const PgStart st = read_start(w.starts[1] + s);
+			end = read_start(w.starts[1] + s + 1);
 			entry = st.entry;
 			kv = st.kv;
 			j1 = st.block;
-			e = read_entry(entries + entry);
+			if (entry >= 0) e = read_entry(entries + entry);
 		}
 	}
 	__device__ bool next() {
 		if (whole) {                     // sorted by length, dealt out forwards and backwards in turn
+			constexpr int slots = PG_TILE_SLOTS;
 			const int i = turn & 1 ? (turn + 1) * slots - 1 - slot : turn * slots + slot;
 			++turn;
-			if (i >= count) return false;
+			if (i / kv_heads >= entry_count) return false;
 			kv = i % kv_heads;
 			e = read_entry(entries + __ldcg(order + i / kv_heads));
 			j0 = 0;
 			j1 = e.blocks;
 			return true;
 		}
-		if (left <= 0) return false;
-		if (turn++ && j1 == e.blocks) {          // the tile before was finished
+		if (entry < 0) return false;
+		if (turn++) {
+			if (j1 < e.blocks) return false;          // the rest is the next slot's
 			j1 = 0;
 			if (++kv == kv_heads) {
 				kv = 0;
-				e = read_entry(entries + ++entry);
+				if (++entry == entry_count) return false;
+				e = read_entry(entries + entry);
 			}
 		}
+		if (end.before(entry, kv)) return false;
 		j0 = j1;
-		j1 = e.blocks - j0 < left ? e.blocks : j0 + left;
-		left -= j1 - j0;
-		return true;
+		j1 = end.in_job(entry, kv) ? end.block : e.blocks;
+		return j0 < j1;
 	}
 };
 
