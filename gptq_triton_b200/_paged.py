@@ -3,6 +3,7 @@ library or a failing kernel raises."""
 from __future__ import annotations
 
 import ctypes
+import threading
 from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
 from typing import Dict, Optional
@@ -52,6 +53,8 @@ _SIGNATURES = {
 
 _lib: Optional[ctypes.CDLL] = None
 _control: Dict[int, torch.Tensor] = {}
+_status: Dict[int, int] = {}
+_lock = threading.Lock()
 
 
 def exported_symbols():
@@ -73,6 +76,28 @@ def lib() -> ctypes.CDLL:
 	return _lib
 
 
+class _Ctypes:
+	"""In the place of the extension module: serves nothing, so every call goes through ctypes."""
+	paged_plan = paged_append = paged_attention = staticmethod(lambda *a: None)
+
+
+_native = None
+
+
+def native():
+	"""The operators in native code (csrc/host/calls.cpp); each returns None when the call is not the plain case."""
+	global _native
+	if _native is None:
+		from . import _lib as base
+		module, l = base.host(), lib()
+		if hasattr(module, 'paged_bind'):
+			module.paged_bind(*(ctypes.cast(getattr(l, name), c_void_p).value for name in ('paged_plan', 'paged_append', 'paged_attention', 'paged_attention_scratch', 'paged_work_ints')))
+			_native = module
+		else:
+			_native = _Ctypes
+	return _native
+
+
 _MESSAGES = {-1: 'invalid argument', -2: 'shape violates a divisibility rule', -3: 'scratch missing or too small', -4: 'pointer or stride misaligned', -5: 'CUDA error', -6: 'not supported'}
 
 
@@ -82,14 +107,19 @@ def check(code: int, what: str):
 		raise (ValueError if code in (-1, -2, -4) else GptqB200Error)(f'{what}: {_MESSAGES.get(code, "unknown error code")}{extra}')
 
 
-def status_ptr(device: torch.device) -> int:
-	"""Address of the status word of the paged operators on `device` (part of _lib.kernel_status())."""
-	index = torch.cuda.current_device() if device.index is None else device.index
-	buf = _control.get(index)
-	if buf is None:
-		if torch.cuda.is_current_stream_capturing():
-			raise GptqB200Error('the first paged operator on a device must run outside of a graph capture: it sets up the status word')
-		buf = _control[index] = torch.zeros(CONTROL_BYTES, dtype=torch.uint8, device=device)
-		torch.cuda.current_stream(device).synchronize()          # (any stream may use it from now on)
-		register_status_buffer(buf)
-	return buf.data_ptr() + CONTROL_BYTES - 4
+def status_ptr(index: int) -> int:
+	"""Address of the status word of the paged operators on device `index` (part of _lib.kernel_status())."""
+	known = _status.get(index)
+	if known is not None:
+		return known
+	with _lock:
+		if index not in _status:
+			if torch.cuda.is_current_stream_capturing():
+				raise GptqB200Error('the first paged operator on a device must run outside of a graph capture: it sets up the status word')
+			device = torch.device('cuda', index)
+			buf = torch.zeros(CONTROL_BYTES, dtype=torch.uint8, device=device)
+			torch.cuda.current_stream(device).synchronize()          # (any stream may use it from now on)
+			register_status_buffer(buf)
+			_control[index] = buf
+			_status[index] = buf.data_ptr() + CONTROL_BYTES - 4
+	return _status[index]

@@ -8,6 +8,9 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <algorithm>
+#include <climits>
+
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
@@ -25,6 +28,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../../include/gptq_b200.h"
+#include "../../../include/paged_b200.h"
 
 namespace {
 
@@ -369,11 +373,259 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
 	return none();
 }
 
+// ---- cache in pages (libpaged_b200.so) ---------------------------------------------------------------------------------------
+decltype(&paged_plan) plan_fn = nullptr;
+decltype(&paged_append) append_fn = nullptr;
+decltype(&paged_attention) attention_fn = nullptr;
+decltype(&paged_attention_scratch) attention_scratch = nullptr;
+decltype(&paged_work_ints) work_ints = nullptr;
+
+// paged_bind(addresses of paged_plan, paged_append, paged_attention, paged_attention_scratch, paged_work_ints)
+PyObject *paged_bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
+	if (n != 5) {
+		PyErr_SetString(PyExc_TypeError, "paged_bind() takes five addresses");
+		return nullptr;
+	}
+	void *p[5];
+	for (int i = 0; i < 5; ++i) {
+		p[i] = PyLong_AsVoidPtr(a[i]);
+		if (PyErr_Occurred()) return nullptr;
+	}
+	plan_fn = reinterpret_cast<decltype(plan_fn)>(p[0]);
+	append_fn = reinterpret_cast<decltype(append_fn)>(p[1]);
+	attention_fn = reinterpret_cast<decltype(attention_fn)>(p[2]);
+	attention_scratch = reinterpret_cast<decltype(attention_scratch)>(p[3]);
+	work_ints = reinterpret_cast<decltype(work_ints)>(p[4]);
+	return none();
+}
+
+at::ScalarType paged_type(int64_t code) { return code == 0 ? at::kBFloat16 : code == 1 ? at::kFloat : at::kHalf; }
+bool count(PyObject *o, int64_t &v) { return integer(o, v) && v >= 0; }
+bool address(PyObject *o, void *&v) {
+	v = PyLong_CheckExact(o) ? PyLong_AsVoidPtr(o) : nullptr;
+	return v && !PyErr_Occurred();
+}
+
+struct Pages {          // a cache tensor
+	const at::Tensor *t = nullptr;
+	bool load(PyObject *o, at::ScalarType type, int device) {
+		t = strided(o, type, device);
+		return t && t->dim() == 4 && t->numel() > 0 && t->stride(3) == 1 && t->stride(2) == t->size(3);
+	}
+};
+
+// A part of `buf` as a tensor of its own (no slicing through the dispatcher).
+at::Tensor part(const at::Tensor &buf, int64_t offset, int64_t n, bool wide) {
+	at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), wide ? caffe2::TypeMeta::Make<int64_t>() : caffe2::TypeMeta::Make<int32_t>());
+	t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+	t.unsafeGetTensorImpl()->set_storage_offset(wide ? offset / 2 : offset);
+	return t;
+}
+
+// paged_plan(past, new, table, cache, type code, rows, heads, pool, head, max_new, status) -> (row_start, lens, positions, slots, head or None, work)
+PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
+	return guarded([&]() -> PyObject * {
+		int64_t code, rows, heads, most;
+		void *status;
+		if (n != 11 || !plan_fn || !count(a[4], code) || !count(a[5], rows) || !count(a[6], heads) || !count(a[9], most) || !address(a[10], status)) return nullptr;
+		Pages cache;
+		if (code > 2 || !cache.load(a[3], paged_type(code), -1)) return nullptr;
+		const int device = cache.t->get_device();
+		if (device != c10::cuda::current_device()) return nullptr;
+		bool ok = true;
+		const at::Tensor *past = plain(a[0], at::kInt, device), *fresh = plain(a[1], at::kInt, device), *table = strided(a[2], at::kInt, device), *pool = maybe(a[7], at::kInt, device, ok),
+						 *head = maybe(a[8], at::kInt, device, ok);
+		if (!ok || !past || !fresh || !table || past->dim() != 1 || fresh->dim() != 1 || table->dim() != 2 || past->numel() == 0 || fresh->numel() != past->numel() || table->size(0) != past->numel() ||
+			table->size(1) < 1 || table->stride(1) != 1 || (table->size(0) > 1 && table->stride(0) < table->size(1)) || !pool != !head || (pool && (pool->dim() != 1 || head->dim() != 1 || head->numel() != 1)) || rows == 0 || most > rows)
+			return nullptr;
+		const int64_t R = past->numel(), pages = cache.t->size(0), kv = cache.t->size(1), page = cache.t->size(2), dim = cache.t->size(3);
+		if (R > PAGED_MAX_REQUESTS || heads < 1 || heads % kv || pages > INT_MAX || page > INT_MAX || table->size(1) > INT_MAX || (pool && pool->numel() > INT_MAX)) return nullptr;
+		const int64_t ints = work_ints((int)R, (int)rows, (int)heads, (int)kv);
+		if (ints < 0) return nullptr;
+		const int64_t at_work = (2 * rows + 3) / 4 * 4, at_start = at_work + ints, at_lens = at_start + R + 1, at_pos = at_lens + R, at_head = at_pos + rows;
+		at::Tensor buf = at::empty({at_head + 1}, at::TensorOptions().dtype(at::kInt).device(cache.t->device()));
+		if (buf.key_set().has(c10::DispatchKey::Python)) return nullptr;
+		int32_t *w = static_cast<int32_t *>(buf.data_ptr());
+		paged_plan_t p = {};
+		p.requests = (int)R;
+		p.rows = (int)rows;
+		p.table_width = (int)table->size(1);
+		p.page = (int)page;
+		p.pages = (int)pages;
+		p.pool_size = pool ? (int)pool->numel() : 0;
+		p.table_ld = std::max(table->stride(0), table->size(1));
+		p.past = words(past);
+		p.fresh = words(fresh);
+		p.table = static_cast<int32_t *>(table->data_ptr());
+		p.pool = words(pool);
+		p.head = words(head);
+		p.next_head = pool ? w + at_head : nullptr;
+		p.row_start = w + at_start;
+		p.lens = w + at_lens;
+		p.positions = w + at_pos;
+		p.slots = reinterpret_cast<int64_t *>(w);
+		p.heads = (int)heads;
+		p.kv_heads = (int)kv;
+		p.dim = (int)dim;
+		p.max_fresh = (int)most;
+		p.work = w + at_work;
+		p.status = static_cast<int *>(status);
+		cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+		int rc;
+		Py_BEGIN_ALLOW_THREADS
+		rc = plan_fn(&p, (int)code, stream);
+		Py_END_ALLOW_THREADS
+		if (rc != GPTQ_OK) return nullptr;
+		PyObject *o[6] = {THPVariable_Wrap(part(buf, at_start, R + 1, false)), THPVariable_Wrap(part(buf, at_lens, R, false)), THPVariable_Wrap(part(buf, at_pos, rows, false)),
+						  THPVariable_Wrap(part(buf, 0, rows, true)), pool ? THPVariable_Wrap(part(buf, at_head, 1, false)) : Py_NewRef(Py_None), THPVariable_Wrap(part(buf, at_work, ints, false))};
+		PyObject *r = PyTuple_New(6);
+		for (int i = 0; i < 6; ++i) PyTuple_SET_ITEM(r, i, o[i]);
+		return r;
+	});
+}
+
+// What the calls of a layer have in common: type code, heads, kv_heads, page, pages, dim, rows of the plan; caches and row tensors that fit.
+struct Layer {
+	int64_t code, heads, kv, page, pages, dim, rows;
+	at::ScalarType type;
+	Pages k, v;
+	int device = -1;
+	bool load(PyObject *const *a) { return count(a[0], code) && count(a[1], heads) && count(a[2], kv) && count(a[3], page) && count(a[4], pages) && count(a[5], dim) && count(a[6], rows) && code <= 2; }
+	bool caches(PyObject *ko, PyObject *vo) {
+		type = paged_type(code);
+		if (!k.load(ko, type, -1)) return false;
+		device = k.t->get_device();
+		if (device != c10::cuda::current_device() || !v.load(vo, type, device)) return false;
+		for (const at::Tensor *t : {k.t, v.t})
+			if (t->size(0) != pages || t->size(1) != kv || t->size(2) != page || t->size(3) != dim) return false;
+		return rows > 0;
+	}
+	const at::Tensor *operand(PyObject *o, int64_t h) const {
+		const at::Tensor *t = strided(o, type, device);
+		return t && t->dim() == 3 && t->size(0) == rows && t->size(1) == h && t->size(2) == dim && t->stride(2) == 1 ? t : nullptr;
+	}
+	at::Tensor result(PyObject *o, bool &ok) const {          // `out`, or a new tensor
+		if (o == Py_None) return at::empty({rows, heads, dim}, at::TensorOptions().dtype(type).device(k.t->device()));
+		const at::Tensor *t = operand(o, heads);
+		ok = t && t->is_contiguous();
+		return ok ? *t : at::Tensor();
+	}
+};
+
+// paged_append(q, k, v, k_cache, v_cache, cos, sin, out, positions, slots, <layer>, status) -> out
+PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+	return guarded([&]() -> PyObject * {
+		Layer l;
+		void *status;
+		if (n != 18 || !append_fn || !l.load(a + 10) || !address(a[17], status) || !l.caches(a[3], a[4])) return nullptr;
+		bool ok = true;
+		const at::Tensor *q = l.operand(a[0], l.heads), *k = l.operand(a[1], l.kv), *v = l.operand(a[2], l.kv), *cos = maybe(a[5], l.type, l.device, ok), *sin = maybe(a[6], l.type, l.device, ok);
+		const at::Tensor *pos = plain(a[8], at::kInt, l.device), *slots = plain(a[9], at::kLong, l.device);
+		if (!ok || !q || !k || !v || !pos || !slots || pos->numel() != l.rows || slots->numel() != l.rows || !cos != !sin) return nullptr;
+		if (cos && (cos->dim() != 2 || !cos->sizes().equals(sin->sizes()) || cos->size(0) < 1 || cos->size(1) > l.dim || cos->size(1) % 2)) return nullptr;
+		at::Tensor out = l.result(a[7], ok);
+		if (!ok || out.key_set().has(c10::DispatchKey::Python)) return nullptr;
+		paged_append_t p = {};
+		p.rows = (int)l.rows;
+		p.heads = (int)l.heads;
+		p.kv_heads = (int)l.kv;
+		p.dim = (int)l.dim;
+		p.rot = cos ? (int)cos->size(1) : 0;
+		p.max_pos = cos ? (int)cos->size(0) : 0;
+		p.page = (int)l.page;
+		p.pages = (int)l.pages;
+		p.q = ptr(q);
+		p.k = ptr(k);
+		p.v = ptr(v);
+		p.q_row = q->stride(0);
+		p.q_head = q->stride(1);
+		p.k_row = k->stride(0);
+		p.k_head = k->stride(1);
+		p.v_row = v->stride(0);
+		p.v_head = v->stride(1);
+		p.cos_t = ptr(cos);
+		p.sin_t = ptr(sin);
+		p.positions = words(pos);
+		p.slots = static_cast<const int64_t *>(ptr(slots));
+		p.q_out = out.data_ptr();
+		p.k_cache = ptr(l.k.t);
+		p.v_cache = ptr(l.v.t);
+		p.k_page = l.k.t->stride(0);
+		p.k_kv = l.k.t->stride(1);
+		p.v_page = l.v.t->stride(0);
+		p.v_kv = l.v.t->stride(1);
+		p.status = static_cast<int *>(status);
+		cudaStream_t stream = c10::cuda::getCurrentCUDAStream(l.device).stream();
+		int rc;
+		Py_BEGIN_ALLOW_THREADS
+		rc = append_fn(&p, (int)l.code, stream);
+		Py_END_ALLOW_THREADS
+		return rc == GPTQ_OK ? THPVariable_Wrap(std::move(out)) : nullptr;
+	});
+}
+
+// paged_attention(q, k_cache, v_cache, out, scale, table, row_start, lens, work, max_new, <layer>, status) -> out
+PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+	return guarded([&]() -> PyObject * {
+		Layer l;
+		void *status;
+		int64_t most;
+		if (n != 18 || !attention_fn || !PyFloat_CheckExact(a[4]) || !count(a[9], most) || !l.load(a + 10) || !address(a[17], status) || !l.caches(a[1], a[2])) return nullptr;
+		bool ok = true;
+		const at::Tensor *q = l.operand(a[0], l.heads), *table = strided(a[5], at::kInt, l.device), *start = plain(a[6], at::kInt, l.device), *lens = plain(a[7], at::kInt, l.device),
+						 *work = plain(a[8], at::kInt, l.device);
+		if (!q || !table || !start || !lens || !work || table->dim() != 2) return nullptr;
+		at::Tensor out = l.result(a[3], ok);
+		if (!ok || out.key_set().has(c10::DispatchKey::Python)) return nullptr;
+		paged_attention_t p = {};
+		p.requests = (int)lens->numel();
+		p.rows = (int)l.rows;
+		p.heads = (int)l.heads;
+		p.kv_heads = (int)l.kv;
+		p.dim = (int)l.dim;
+		p.page = (int)l.page;
+		p.pages = (int)l.pages;
+		p.table_width = (int)table->size(1);
+		p.max_fresh = (int)most;
+		p.table_ld = std::max(table->stride(0), table->size(1));
+		p.scale = (float)PyFloat_AS_DOUBLE(a[4]);
+		p.q = ptr(q);
+		p.q_row = q->stride(0);
+		p.q_head = q->stride(1);
+		p.k_cache = ptr(l.k.t);
+		p.v_cache = ptr(l.v.t);
+		p.k_page = l.k.t->stride(0);
+		p.k_kv = l.k.t->stride(1);
+		p.v_page = l.v.t->stride(0);
+		p.v_kv = l.v.t->stride(1);
+		p.table = words(table);
+		p.row_start = words(start);
+		p.lens = words(lens);
+		p.work = words(work);
+		p.out = out.data_ptr();
+		p.status = static_cast<int *>(status);
+		const int64_t need = attention_scratch(&p, (int)l.code);
+		if (need < 0) return nullptr;
+		const at::Tensor scratch = at::empty({need}, at::TensorOptions().dtype(at::kByte).device(q->device()));
+		if (scratch.key_set().has(c10::DispatchKey::Python)) return nullptr;
+		p.scratch = scratch.data_ptr();
+		p.scratch_bytes = need;
+		cudaStream_t stream = c10::cuda::getCurrentCUDAStream(l.device).stream();
+		int rc;
+		Py_BEGIN_ALLOW_THREADS
+		rc = attention_fn(&p, (int)l.code, stream);
+		Py_END_ALLOW_THREADS
+		return rc == GPTQ_OK ? THPVariable_Wrap(std::move(out)) : nullptr;
+	});
+}
+
 template <typename F>
 PyCFunction fast(F f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)); }
 
 PyMethodDef methods[] = {{"bind", fast(bind), METH_FASTCALL, nullptr}, {"qmatmul", fast(qmatmul), METH_FASTCALL, nullptr}, {"gateup", fast(gateup), METH_FASTCALL, nullptr},
-						 {"qkv", fast(qkv), METH_FASTCALL, nullptr}, {"attend", fast(attend), METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
+						 {"qkv", fast(qkv), METH_FASTCALL, nullptr}, {"attend", fast(attend), METH_FASTCALL, nullptr},
+						 {"paged_bind", fast(paged_bind), METH_FASTCALL, nullptr}, {"paged_plan", fast(plan), METH_FASTCALL, nullptr},
+						 {"paged_append", fast(append), METH_FASTCALL, nullptr}, {"paged_attention", fast(attention), METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }   // namespace

@@ -80,6 +80,13 @@ def paged_plan(past: torch.Tensor, new: torch.Tensor, table: torch.Tensor, cache
 	cache: a key cache tensor of the layers, for its sizes and type.  rows: rows of q, k and v, at least the sum of `new`; rows left over
 	get slot -1.  heads: query heads.  max_new: no request has more new tokens (default: rows); only speed depends on it.
 	"""
+	if cache.is_cuda:
+		code = _paged.DTYPE_CODE.get(cache.dtype)
+		served = _paged.native().paged_plan(past, new, table, cache, code, rows, heads, pool, head, rows if max_new is None else min(max_new, rows), _paged.status_ptr(cache.get_device()))
+		if served is not None:
+			row_start, lens, positions, slots, nxt, work = served
+			pages, kv_heads, page, dim = cache.shape
+			return PagedPlan(table, row_start, lens, positions, slots, nxt, work, rows, rows if max_new is None else min(max_new, rows), (heads, kv_heads, page, pages, dim, cache.dtype))
 	require_cuda(past, new, table, cache, pool, head)
 	dev = cache.device
 	_cache(cache, 'cache')
@@ -117,7 +124,7 @@ def paged_plan(past: torch.Tensor, new: torch.Tensor, table: torch.Tensor, cache
 	a.table_ld = max(table.stride(0), table.shape[1])
 	a.past, a.fresh, a.table, a.pool, a.head = ptr(past), ptr(new), ptr(table), ptr(pool), ptr(head)
 	a.next_head, a.row_start, a.lens, a.positions, a.slots = ptr(nxt) if pool is not None else None, ptr(row_start), ptr(lens), ptr(positions), ptr(slots)
-	a.heads, a.kv_heads, a.dim, a.max_fresh, a.work, a.status = heads, kv_heads, dim, max_new, ptr(work), _paged.status_ptr(dev)
+	a.heads, a.kv_heads, a.dim, a.max_fresh, a.work, a.status = heads, kv_heads, dim, max_new, ptr(work), _paged.status_ptr(dev.index)
 	with _On(dev):
 		_paged.check(lib.paged_plan(ctypes.byref(a), _paged.DTYPE_CODE[cache.dtype], stream_ptr(dev)), 'paged_plan')
 	return PagedPlan(table, row_start, lens, positions, slots, None if pool is None else nxt, work, rows, max_new, (heads, kv_heads, page, pages, dim, cache.dtype))
@@ -155,9 +162,14 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: tor
 	only; without tables nothing is turned.  Rows with slot -1 are not stored; a position outside the tables sets status 4, its row is
 	turned as position 0 and not stored.  `out` may be q itself (contiguous).
 	"""
+	heads, kv_heads, page, pages, dim, dt = plan.serves
+	if q.is_cuda:
+		served = _paged.native().paged_append(q, k, v, k_cache, v_cache, cos, sin, out, plan.positions, plan.slots, _paged.DTYPE_CODE[dt], heads, kv_heads, page, pages, dim, plan.rows,
+											  _paged.status_ptr(q.get_device()))
+		if served is not None:
+			return served
 	require_cuda(q, k, v, k_cache, v_cache, cos, sin, out)
 	_caches(k_cache, v_cache, plan, 'paged_append')
-	heads, kv_heads, page, pages, dim, dt = plan.serves
 	_rows(q, 'q', plan, heads)
 	_rows(k, 'k', plan, kv_heads)
 	_rows(v, 'v', plan, kv_heads)
@@ -177,7 +189,7 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: tor
 	a.q, a.k, a.v = ptr(q), ptr(k), ptr(v)
 	a.q_row, a.q_head, a.k_row, a.k_head, a.v_row, a.v_head = q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1)
 	a.positions, a.slots, a.q_out, a.k_cache, a.v_cache = ptr(plan.positions), ptr(plan.slots), ptr(res), ptr(k_cache), ptr(v_cache)
-	a.k_page, a.k_kv, a.v_page, a.v_kv, a.status = k_cache.stride(0), k_cache.stride(1), v_cache.stride(0), v_cache.stride(1), _paged.status_ptr(dev)
+	a.k_page, a.k_kv, a.v_page, a.v_kv, a.status = k_cache.stride(0), k_cache.stride(1), v_cache.stride(0), v_cache.stride(1), _paged.status_ptr(dev.index)
 	with _On(dev):
 		_paged.check(_paged.lib().paged_append(ctypes.byref(a), _paged.DTYPE_CODE[dt], stream_ptr(dev)), 'paged_append')
 	return res
@@ -190,16 +202,21 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 	Rows behind the last one in use are left as they are (`out`) or have no particular value.  Values of positions behind a request's last
 	one do not count, whatever the pages hold there.
 	"""
+	heads, kv_heads, page, pages, dim, dt = plan.serves
+	scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+	if q.is_cuda:
+		served = _paged.native().paged_attention(q, k_cache, v_cache, out, scale, plan.table, plan.row_start, plan.lens, plan.work, plan.max_new, _paged.DTYPE_CODE[dt], heads, kv_heads, page,
+												 pages, dim, plan.rows, _paged.status_ptr(q.get_device()))
+		if served is not None:
+			return served
 	require_cuda(q, k_cache, v_cache, out)
 	_caches(k_cache, v_cache, plan, 'paged_attention')
-	heads, kv_heads, page, pages, dim, dt = plan.serves
 	_rows(q, 'q', plan, heads)
 	dev = q.device
 	if k_cache.device != dev or v_cache.device != dev:
 		raise ValueError('paged_attention: caches and queries must be on one device')
 	if dim % 8 or dim > _paged.MAX_DIM:
 		raise ValueError(f'paged_attention serves head sizes that are multiples of 8 up to {_paged.MAX_DIM}, not {dim}')
-	scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
 	if not (0.0 < scale < math.inf):
 		raise ValueError('scale must be positive and finite')
 	res = _out(out, q)
@@ -209,7 +226,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 	a.table_ld, a.scale = max(plan.table.stride(0), plan.table.shape[1]), scale
 	a.q, a.q_row, a.q_head, a.k_cache, a.v_cache = ptr(q), q.stride(0), q.stride(1), ptr(k_cache), ptr(v_cache)
 	a.k_page, a.k_kv, a.v_page, a.v_kv = k_cache.stride(0), k_cache.stride(1), v_cache.stride(0), v_cache.stride(1)
-	a.table, a.row_start, a.lens, a.work, a.out, a.status = ptr(plan.table), ptr(plan.row_start), ptr(plan.lens), ptr(plan.work), ptr(res), _paged.status_ptr(dev)
+	a.table, a.row_start, a.lens, a.work, a.out, a.status = ptr(plan.table), ptr(plan.row_start), ptr(plan.lens), ptr(plan.work), ptr(res), _paged.status_ptr(dev.index)
 	need = lib.paged_attention_scratch(ctypes.byref(a), code)
 	scratch = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
 	a.scratch, a.scratch_bytes = ptr(scratch), scratch.numel()
