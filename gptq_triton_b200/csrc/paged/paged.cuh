@@ -52,6 +52,7 @@ struct PgEntry {
 };
 struct PgStart {                       // entry -1: behind the last job
 	int entry, kv, block, pad;
+	PgEntry job;                        // entries[entry]
 	__device__ bool in_job(int e, int k) const { return entry == e && kv == k; }
 	__device__ bool before(int e, int k) const { return entry >= 0 && (entry < e || (entry == e && kv < k)); }          // its job comes before
 };
@@ -63,8 +64,8 @@ __device__ __forceinline__ PgList read_list(const PgList *p) {
 	return PgList{a.x, a.y, b, c};
 }
 __device__ __forceinline__ PgStart read_start(const PgStart *p) {
-	const int4 a = __ldcg(reinterpret_cast<const int4 *>(p));
-	return PgStart{a.x, a.y, a.z, a.w};
+	const int4 a = __ldcg(reinterpret_cast<const int4 *>(p)), b = __ldcg(reinterpret_cast<const int4 *>(p) + 1), c = __ldcg(reinterpret_cast<const int4 *>(p) + 2);
+	return PgStart{a.x, a.y, a.z, a.w, PgEntry{b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w}};
 }
 __device__ __forceinline__ PgEntry read_entry(const PgEntry *p) {
 	const int4 a = __ldcg(reinterpret_cast<const int4 *>(p)), b = __ldcg(reinterpret_cast<const int4 *>(p) + 1);
@@ -87,9 +88,9 @@ inline __host__ __device__ PgWork pg_work(int32_t *base, int requests, int rows,
 	int64_t at = 16;
 	w.list = reinterpret_cast<PgList *>(base);
 	w.starts[0] = reinterpret_cast<PgStart *>(base + at);
-	at += 4 * (PG_SLOTS + 1);
+	at += 12 * (PG_SLOTS + 1);
 	w.starts[1] = reinterpret_cast<PgStart *>(base + at);
-	at += 4 * (PG_TILE_SLOTS + 1);
+	at += 12 * (PG_TILE_SLOTS + 1);
 	w.entries[0] = reinterpret_cast<PgEntry *>(base + at);
 	at += 8 * (int64_t)w.cap[0];
 	w.entries[1] = reinterpret_cast<PgEntry *>(base + at);
@@ -107,6 +108,7 @@ inline bool pg_tiles_serve(int dtype, int dim, int page, int max_fresh, int head
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, int bytes) {
 	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ float ex2(float x) {
 	float r;
 	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

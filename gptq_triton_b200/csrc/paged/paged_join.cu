@@ -13,31 +13,31 @@ constexpr int JN_THREADS = 128, JN_ROWS = 16;            // rows of a tile that 
 template <typename T> __device__ __forceinline__ void store_four(T *dst, float4 v) { *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w)); }
 template <> __device__ __forceinline__ void store_four<float>(float *dst, float4 v) { *reinterpret_cast<float4 *>(dst) = v; }
 
-// kind 0: tiles of PG_ROWS rows, 1: of PG_TILE rows; DP: columns of a partial result
-template <typename T, int DP>
-__device__ void join(const paged_attention_t &p, const PgWork &work, int kind, int slot, int row0, const float *scratch) {
-	const int group = p.heads / p.kv_heads, tile_rows = kind ? PG_TILE : PG_ROWS, slots = kind ? PG_TILE_SLOTS : PG_SLOTS;
-	if (read_list(work.list + kind).whole) return;
+// kind 0: tiles of PG_ROWS rows, 1: of PG_TILE rows; DP: columns of a partial result.  Further slots that the job which begins in `slot`
+// runs through (0: there is none), and its start in the next one.
+__device__ __forceinline__ int cut(const PgWork &work, int kind, int slot, PgStart &s) {
+	const int slots = kind ? PG_TILE_SLOTS : PG_SLOTS;
+	if (read_list(work.list + kind).whole) return 0;
 	const PgStart *starts = work.starts[kind];
-	const PgStart s = read_start(starts + slot + 1), before = read_start(starts + slot);
-	if (s.entry < 0 || s.block == 0 || (before.in_job(s.entry, s.kv) && before.block > 0)) return;
-	const PgEntry e = read_entry(work.entries[kind] + s.entry);
-	if (row0 >= (int64_t)e.fresh * group - (int64_t)e.tile * tile_rows) return;
-	// further slots that begin inside the job
-	int more = 1;
-	for (;; more += 32) {
+	s = read_start(starts + slot + 1);
+	const PgStart before = read_start(starts + slot);
+	if (s.entry < 0 || s.block == 0 || (before.in_job(s.entry, s.kv) && before.block > 0)) return 0;
+	for (int more = 1;; more += 32) {
 		const int c = slot + 1 + more + (threadIdx.x & 31);
 		bool inside = false;
 		if (c <= slots) {
-			const PgStart n = read_start(starts + c);
-			inside = n.in_job(s.entry, s.kv) && n.block > 0;
+			const int4 n = __ldcg(reinterpret_cast<const int4 *>(starts + c));
+			inside = n.x == s.entry && n.y == s.kv && n.z > 0;
 		}
 		const unsigned gone = ~__ballot_sync(0xffffffffu, inside);
-		if (gone) {
-			more += __ffs(gone) - 1;
-			break;
-		}
+		if (gone) return more + __ffs(gone) - 1;
 	}
+}
+
+template <typename T, int DP>
+__device__ void join(const paged_attention_t &p, int kind, int slot, int row0, const float *scratch, const PgStart &s, int more) {
+	const int group = p.heads / p.kv_heads, tile_rows = kind ? PG_TILE : PG_ROWS;
+	const PgEntry &e = s.job;
 	auto part = [&](int i) { return scratch + (int64_t)(i == 0 ? 2 * slot + 1 : 2 * (slot + i)) * tile_rows * (DP + 2); };
 	for (int x = threadIdx.x; x < JN_ROWS * (DP / 4); x += JN_THREADS) {
 		const int row = row0 + x / (DP / 4), col = x % (DP / 4) * 4;
@@ -81,14 +81,15 @@ __device__ void join(const paged_attention_t &p, const PgWork &work, int kind, i
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(JN_THREADS) join_kernel(const paged_attention_t p, const PgWork work, const float *tile_scratch) {
+	const bool few = blockIdx.x < PG_SLOTS;
+	const int x = blockIdx.x - (few ? 0 : PG_SLOTS), slot = few ? x : x % PG_TILE_SLOTS;
+	PgStart s;
+	const int more = cut(work, few ? 0 : 1, slot, s);      // (the plan was complete before the attention kernels could start this one)
 	pdl_wait();
 	pdl_trigger();
-	if (blockIdx.x < PG_SLOTS) {
-		join<T, DP>(p, work, 0, blockIdx.x, 0, reinterpret_cast<const float *>(p.scratch));
-	} else if (DP <= 128) {
-		const int x = blockIdx.x - PG_SLOTS;
-		join<T, DP>(p, work, 1, x % PG_TILE_SLOTS, x / PG_TILE_SLOTS * JN_ROWS, tile_scratch);
-	}
+	if (more == 0) return;
+	if (few) join<T, DP>(p, 0, slot, 0, reinterpret_cast<const float *>(p.scratch), s, more);
+	else if (DP <= 128) join<T, DP>(p, 1, slot, x / PG_TILE_SLOTS * JN_ROWS, tile_scratch, s, more);
 }
 
 template <typename T>

@@ -84,7 +84,7 @@ __device__ __forceinline__ Lengths lengths_of(const paged_plan_t &p, int r, int 
 // What the attention sees of a request is at most what its table can name.
 __device__ __forceinline__ int length_seen(const paged_plan_t &p, const Lengths &l) { return (int)min((int64_t)l.past + l.fresh, min((int64_t)p.table_width * p.page, (int64_t)PL_LIMIT)); }
 
-constexpr int PL_JOIN = 6;
+constexpr int PL_JOIN = 6, PL_LEAST = 2;
 constexpr int PL_KEEP = 4096;          // units before an entry that are kept in shared memory for the search
 
 // The work list of one kernel.  s_tiles [R + 1]: tiles of the requests before; s_first: PL_KEEP ints.
@@ -118,9 +118,9 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 		units = add_to(units, total, PL_LIMIT);
 	}
 	__syncthreads();
-	// (a share is longer than what a job costs besides its blocks, so that no two slots begin at the same place; shares of less than
-	// four blocks would be mostly partial results)
-	const int64_t total = (int64_t)units * p.kv_heads, per = max((total + slots - 1) / slots, (int64_t)(4 + pg_begin(kind)));
+	// (a share is longer than what a job costs besides its blocks, so that no two slots begin at the same place; shorter
+	// shares would be mostly partial results)
+	const int64_t total = (int64_t)units * p.kv_heads, per = max((total + slots - 1) / slots, (int64_t)(PL_LEAST + pg_begin(kind)));
 	int whole = 0;
 	if (kind) {
 		// Whole tiles, the longest first, dealt out to the slots forwards and backwards in turn, unless the longest slot would then work
@@ -157,7 +157,7 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 	if (tid == 0) w.list[kind] = PgList{E, whole, per, total};
 	for (int c = tid; c <= slots; c += PL_THREADS) {
 		const int64_t u = c * per;
-		PgStart s = {-1, 0, 0, 0};
+		PgStart s = {-1, 0, 0, 0, {}};
 		if (u < total) {
 			const int x = (int)(u / p.kv_heads);
 			int e;
@@ -172,8 +172,9 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 				}
 				e = lo;
 			}
-			const int n = w.entries[kind][e].blocks + pg_begin(kind);
-			const int64_t rest = u - (int64_t)w.entries[kind][e].first * p.kv_heads;
+			s.job = w.entries[kind][e];
+			const int n = s.job.blocks + pg_begin(kind);
+			const int64_t rest = u - (int64_t)s.job.first * p.kv_heads;
 			s.entry = e;
 			s.kv = (int)(rest / n);
 			s.block = max((int)(rest % n) - pg_begin(kind), 0);

@@ -76,12 +76,12 @@ template <int DP> struct RowsShape {
 struct Walk {                          // a block of a slot's jobs
 	int entry, kv, block;
 	PgEntry e;
-	__device__ __forceinline__ bool start(const PgStart &s, const PgStart &end, const PgEntry *entries) {
+	__device__ __forceinline__ bool start(const PgStart &s, const PgStart &end) {
 		entry = s.entry;
 		kv = s.kv;
 		block = s.block;
 		if (entry < 0 || (end.in_job(entry, kv) && end.block <= block)) return false;
-		e = read_entry(entries + entry);
+		e = s.job;
 		return true;
 	}
 	__device__ __forceinline__ bool step(const PgStart &end, const PgEntry *entries, int entry_count, int kv_heads) {          // false: no block is left
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 	using S = RowsShape<DP>;
 	extern __shared__ __align__(128) unsigned char rw_smem[];
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
-	constexpr float LIFT = std::is_same<T, __half>::value ? 14.f : 0.f;          // fp16 weights up to 2^14: small ones stay above its subnormal range
+	constexpr float LIFT = std::is_same<T, __half>::value ? 7.f : 0.f;          // fp16 weights up to 2^15: small ones stay above its subnormal range
 	// Beside the tile kernel this one needs nothing of it and runs as soon as SMs are free: what came before the tile kernel is complete
 	// when that triggers, and the wait is at the end, so that whoever waits for this kernel waits for both.
 	if (!beside) pdl_wait();
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 	const int entry_count = read_list(work.list).entries;
 	const PgStart begin = read_start(work.starts[0] + slot), end = read_start(work.starts[0] + slot + 1);
 	Walk at;
-	if (!at.start(begin, end, entries)) {
+	if (!at.start(begin, end)) {
 		if (beside) pdl_wait();
 		return;
 	}
@@ -150,6 +150,15 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 				k += next_id * p.k_page + ahead.kv * p.k_kv + first;
 				v += next_id * p.v_page + ahead.kv * p.v_kv + first;
 			}
+			const uint32_t base = dst + sub * DP * 2 + ((unit ^ sub) << 4);          // (ROWS divides 8: row r + sub is swizzled by r ^ sub)
+			if (rows == PG_KEYS && units == S::UNITS) {
+#pragma unroll
+				for (int r = 0; r < PG_KEYS; r += ROWS) {
+					const uint32_t to = (base ^ ((r & 7) << 4)) + r * DP * 2;
+					cp_async16(to, k + sub * DP + r * DP);
+					cp_async16(to + S::HALF, v + sub * DP + r * DP);
+				}
+			} else
 #pragma unroll
 			for (int r = 0; r < PG_KEYS; r += ROWS) {
 				const int row = r + sub;
@@ -218,14 +227,19 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 		const uint32_t sk = ring + (uint32_t)stage * 2 * S::HALF, sv = sk + S::HALF;
 		const int key0 = at.block * PG_KEYS;
 		{
-			float s[2][4] = {};
+			// two chains of MMAs per eight keys
+			float s[2][4] = {}, s2[2][4] = {};
 			const int kr = (lane >> 4) * 8 + (lane & 7), ku = (lane >> 3) & 1;
+			const uint32_t ka = sk + kr * DP * 2 + ((ku ^ (kr & 7)) << 4);          // (16-byte units are swizzled by their row: unit 2 k + ku lies at this address ^ 32 k)
 #pragma unroll
-			for (int k = 0; k < DP / 16; ++k) {
-				uint32_t b[4];
-				ldsm4(b, sk + kr * DP * 2 + (((2 * k + ku) ^ (kr & 7)) << 4));
+			for (int k = 0; k < DP / 16; k += 2) {
+				uint32_t b[4], c[4];
+				ldsm4(b, ka ^ (32 * k));
+				ldsm4(c, ka ^ (32 * k + 32));
 				mma16<T>(s[0], q[k], b[0], b[1]);
 				mma16<T>(s[1], q[k], b[2], b[3]);
+				mma16<T>(s2[0], q[k + 1], c[0], c[1]);
+				mma16<T>(s2[1], q[k + 1], c[2], c[3]);
 			}
 			const bool edge = key0 + PG_KEYS > least;
 			float top[2];
@@ -236,19 +250,19 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 #pragma unroll
 					for (int j = 0; j < 2; ++j) {
 						float &x = s[t][2 * i + j];
-						x *= to_base2;
+						x = (x + s2[t][2 * i + j]) * to_base2;
 						if (edge && key0 + 8 * t + 2 * tig + j >= seen[i]) x = -INFINITY;
 					}
 				float m = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
 				m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-				m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-				top[i] = fmaxf(m, mx[i]);
+				top[i] = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
 			}
-			if (__any_sync(0xffffffffu, top[0] > mx[0] || top[1] > mx[1])) {
+			// the reference point of a row follows its maximum only when that has grown by more than 2^8
+			if (__any_sync(0xffffffffu, top[0] > mx[0] + 8.f || top[1] > mx[1] + 8.f)) {
 #pragma unroll
 				for (int i = 0; i < 2; ++i) {
-					const float keep = mx[i] == -INFINITY ? 0.f : ex2(mx[i] - top[i]);
-					mx[i] = top[i];
+					const float next = fmaxf(mx[i], top[i]), keep = mx[i] == -INFINITY ? 0.f : ex2(mx[i] - next);
+					mx[i] = next;
 					sum[i] *= keep;
 #pragma unroll
 					for (int t = 0; t < DP / 8; ++t) {
@@ -268,10 +282,11 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 				w[2 + i] = pack2<T>(c, d);
 			}
 			const int vr = ((lane >> 3) & 1) * 8 + (lane & 7), vu = lane >> 4;
+			const uint32_t va = sv + vr * DP * 2 + ((vu ^ (vr & 7)) << 4);
 #pragma unroll
 			for (int t = 0; t < DP / 16; ++t) {
 				uint32_t b[4];
-				ldsm4_t(b, sv + vr * DP * 2 + (((2 * t + vu) ^ (vr & 7)) << 4));
+				ldsm4_t(b, va ^ (32 * t));
 				mma16<T>(o[2 * t], w, b[0], b[1]);
 				mma16<T>(o[2 * t + 1], w, b[2], b[3]);
 			}

@@ -98,7 +98,7 @@ struct Items {
 			entry = st.entry;
 			kv = st.kv;
 			j1 = st.block;
-			if (entry >= 0) e = read_entry(entries + entry);
+			e = st.job;
 		}
 	}
 	__device__ bool next() {
