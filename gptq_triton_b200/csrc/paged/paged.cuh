@@ -46,11 +46,11 @@ struct PgList {                        // of one of the two kernels; behind it i
 	int whole;                          // slots take whole jobs by `order` instead (tile kernel)
 	int64_t per, total;                 // length of a slot's share, of all jobs
 };
-struct PgEntry {
+struct alignas(16) PgEntry {
 	int request, tile, blocks, first;   // blocks of keys that the tile sees; length of the entries before, per key head
 	int row, fresh, len, seen;          // first row and new tokens of the request, its tokens, those that the tile's last row sees
 };
-struct PgStart {                       // entry -1: behind the last job
+struct alignas(16) PgStart {                       // entry -1: behind the last job
 	int entry, kv, block, pad;
 	PgEntry job;                        // entries[entry]
 	__device__ bool in_job(int e, int k) const { return entry == e && kv == k; }

@@ -1,7 +1,7 @@
 // Block tables, slot maps, positions and row offsets of a step from the request lengths, and the distribution of the attention's work.
 //
 // Every CTA scans the lengths of all requests into shared memory for itself (two sums per request: rows and pages taken), which is
-// cheaper than a second launch or a barrier over the grid; then CTA 0 lays out the attention's work, the others write pages and rows.
+// cheaper than a second launch or a barrier over the grid; then two or three lay out the attention's work, the others write pages and rows.
 // A row finds its request by bisection in shared memory.  Table entries that are read (pages of old tokens) and written (pages taken
 // now) are different ones, so the order of the CTAs does not matter, and a second run over the same inputs writes the same.
 // The bytes are nothing; what counts is the chain launch - lengths - scan - table entry - store.
@@ -85,10 +85,14 @@ __device__ __forceinline__ Lengths lengths_of(const paged_plan_t &p, int r, int 
 __device__ __forceinline__ int length_seen(const paged_plan_t &p, const Lengths &l) { return (int)min((int64_t)l.past + l.fresh, min((int64_t)p.table_width * p.page, (int64_t)PL_LIMIT)); }
 
 constexpr int PL_JOIN = 6, PL_LEAST = 2;
-constexpr int PL_KEEP = 4096;          // units before an entry that are kept in shared memory for the search
+constexpr int PL_KEEP = 4096;          // entries whose places and lengths are kept in shared memory
+constexpr int PL_NEAR = 1024;          // ... and those that are kept there whole
+constexpr int PL_PARTS = 2;            // CTAs that share the starts of the kernel for few rows
 
-// The work list of one kernel.  s_tiles [R + 1]: tiles of the requests before; s_first: PL_KEEP ints.
-__device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, const int *s_tiles, int *s_first, int *s_scan, PgWork w) {
+// The work list of one kernel.  s_tiles [R + 1]: tiles of the requests before; s_len [R]; s_entry [PL_NEAR], s_first, s_sorted [PL_KEEP].
+// The CTAs that share a list all form it, `part` 0 writes the entries, each its part of the starts.
+__device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, const int *s_start, const int *s_len, const int *s_tiles, PgEntry *s_entry, int *s_first, int *s_sorted, int *s_scan,
+						PgWork w) {
 	const int tid = threadIdx.x, R = p.requests, tile_rows = kind ? PG_TILE : PG_ROWS, keys = kind ? PG_TILE_KEYS : PG_KEYS, group = p.heads / p.kv_heads;
 	const int slots = kind ? PG_TILE_SLOTS : PG_SLOTS;
 	const int E = min(s_tiles[R], w.cap[kind]);
@@ -96,13 +100,13 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 	for (int base = 0; base < E; base += PL_THREADS) {
 		const int e = base + tid;
 		PgEntry x = {};
-		int bad = 0, n = 0, none = 0;
+		int n = 0, none = 0;
 		if (e < E) {
 			x.request = find(s_tiles, R, e);
 			x.tile = e - s_tiles[x.request];
 			x.row = s_start[x.request];
 			x.fresh = s_start[x.request + 1] - x.row;
-			x.len = length_seen(p, lengths_of(p, x.request, bad));
+			x.len = s_len[x.request];
 			const int last = (int)((min((int64_t)x.fresh * group, (int64_t)(x.tile + 1) * tile_rows) - 1) / group);
 			x.seen = min(max(x.len - x.fresh + last + 1, 0), x.len);
 			x.blocks = max((x.seen + keys - 1) / keys, 1);
@@ -112,12 +116,20 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 		scan2(n, none, PL_LIMIT, PL_LIMIT, total, unused, s_scan);
 		if (e < E) {
 			x.first = add_to(units, n, PL_LIMIT);
-			w.entries[kind][e] = x;
+			if (part == 0) {
+				int4 *dst = reinterpret_cast<int4 *>(w.entries[kind] + e);
+				dst[0] = make_int4(x.request, x.tile, x.blocks, x.first);
+				dst[1] = make_int4(x.row, x.fresh, x.len, x.seen);
+			}
+			if (e < PL_NEAR) s_entry[e] = x;
 			if (e < PL_KEEP) s_first[e] = x.first;
 		}
 		units = add_to(units, total, PL_LIMIT);
 	}
 	__syncthreads();
+	if (E > PL_NEAR && part > 0) return;                   // (the other entries are in global memory, where part 0 has written them)
+	if (E > PL_NEAR) parts = 1;
+	auto blocks_of = [&](int e) { return e < PL_NEAR ? s_entry[e].blocks : w.entries[kind][e].blocks; };
 	// (a share is longer than what a job costs besides its blocks, so that no two slots begin at the same place; shorter
 	// shares would be mostly partial results)
 	const int64_t total = (int64_t)units * p.kv_heads, per = max((total + slots - 1) / slots, (int64_t)(PL_LEAST + pg_begin(kind)));
@@ -130,17 +142,23 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 		s_hist[tid] = 0;
 		__syncthreads();
 		if (E <= PL_KEEP) {
-			for (int e = tid; e < E; e += PL_THREADS) atomicMax(&s_most, w.entries[1][e].blocks);
+			int most = 0;
+			for (int e = tid; e < E; e += PL_THREADS) most = max(most, blocks_of(e));
+			atomicMax(&s_most, most);
 			__syncthreads();
 			auto bucket = [&](int n) { return PL_THREADS - 1 - (int)((int64_t)n * (PL_THREADS - 1) / s_most); };
-			for (int e = tid; e < E; e += PL_THREADS) atomicAdd(&s_hist[bucket(w.entries[1][e].blocks)], 1);
+			for (int e = tid; e < E; e += PL_THREADS) atomicAdd(&s_hist[bucket(blocks_of(e))], 1);
 			__syncthreads();
 			int a = s_hist[tid], b = 0, ta, tb;
 			scan2(a, b, PL_LIMIT, PL_LIMIT, ta, tb, s_scan);
 			s_hist[tid] = a;
 			__syncthreads();
 			// (tiles of one length are in no particular order: which slot takes one changes no result)
-			for (int e = tid; e < E; e += PL_THREADS) w.order[atomicAdd(&s_hist[bucket(w.entries[1][e].blocks)], 1)] = e;
+			for (int e = tid; e < E; e += PL_THREADS) {
+				const int n = blocks_of(e), at = atomicAdd(&s_hist[bucket(n)], 1);
+				w.order[at] = e;
+				s_sorted[at] = n + pg_begin(1);
+			}
 		} else {
 			for (int e = tid; e < E; e += PL_THREADS) w.order[e] = e;
 		}
@@ -148,18 +166,23 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 		const int64_t items = (int64_t)E * p.kv_heads;
 		if (tid < slots) {
 			int64_t sum = 0;
-			for (int64_t turn = 0, i = tid; i < items; ++turn, i = turn & 1 ? (turn + 1) * slots - 1 - tid : turn * slots + tid) sum += w.entries[1][w.order[i / p.kv_heads]].blocks + pg_begin(1);
+			for (int64_t turn = 0, i = tid; i < items; ++turn, i = turn & 1 ? (turn + 1) * slots - 1 - tid : turn * slots + tid) {
+				const int at = items < PL_LIMIT ? (int)i / p.kv_heads : (int)(i / p.kv_heads);
+				sum += E <= PL_KEEP ? s_sorted[at] : w.entries[1][at].blocks + pg_begin(1);
+			}
 			atomicMax(&s_span, (int)min(sum, (int64_t)PL_LIMIT));
 		}
 		__syncthreads();
 		whole = s_span <= per + PL_JOIN;
 	}
-	if (tid == 0) w.list[kind] = PgList{E, whole, per, total};
-	for (int c = tid; c <= slots; c += PL_THREADS) {
+	if (tid == 0 && part == 0) w.list[kind] = PgList{E, whole, per, total};
+	if (whole) return;                                     // (nobody looks at the starts)
+	for (int c = part * PL_THREADS + tid; c <= slots; c += parts * PL_THREADS) {
 		const int64_t u = c * per;
 		PgStart s = {-1, 0, 0, 0, {}};
 		if (u < total) {
-			const int x = (int)(u / p.kv_heads);
+			const bool small = total < PL_LIMIT;
+			const int x = small ? (int)u / p.kv_heads : (int)(u / p.kv_heads);
 			int e;
 			if (E <= PL_KEEP) {
 				e = find(s_first, E, x);
@@ -172,20 +195,22 @@ __device__ void lay_out(const paged_plan_t &p, int kind, const int *s_start, con
 				}
 				e = lo;
 			}
-			s.job = w.entries[kind][e];
+			s.entry = e;
+			s.job = e < PL_NEAR ? s_entry[e] : w.entries[kind][e];
 			const int n = s.job.blocks + pg_begin(kind);
 			const int64_t rest = u - (int64_t)s.job.first * p.kv_heads;
-			s.entry = e;
-			s.kv = (int)(rest / n);
-			s.block = max((int)(rest % n) - pg_begin(kind), 0);
+			s.kv = small ? (int)rest / n : (int)(rest / n);
+			s.block = max((int)(rest - (int64_t)s.kv * n) - pg_begin(kind), 0);
 		}
-		w.starts[kind][c] = s;
+		int4 *dst = reinterpret_cast<int4 *>(w.starts[kind] + c);          // (16 bytes at a time: word by word these stores take half of the kernel's time)
+		dst[0] = make_int4(s.entry, s.kv, s.block, 0);
+		dst[1] = make_int4(s.job.request, s.job.tile, s.job.blocks, s.job.first);
+		dst[2] = make_int4(s.job.row, s.job.fresh, s.job.len, s.job.seen);
 	}
-	__syncthreads();
 }
 
 __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, int tiles) {
-	extern __shared__ int pl_smem[];
+	extern __shared__ __align__(16) int pl_smem[];
 	__shared__ int s_scan[64];
 	int *s_start = pl_smem, *s_off = pl_smem + p.requests + 1;
 	const int tid = threadIdx.x, R = p.requests;
@@ -227,18 +252,24 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, 
 		return id;
 	};
 
-	if (blockIdx.x == 0) {
+	const int planners = PL_PARTS + (tiles ? 1 : 0);
+	if ((int)blockIdx.x < planners) {
 		for (int r = tid; r < R; r += PL_THREADS) {
 			const Lengths l = lengths_of(p, r, bad);
-			p.row_start[r] = s_start[r];
-			p.lens[r] = length_seen(p, l);
-			if (p.lens[r] < l.past + l.fresh) bad |= PAGED_NO_ROOM;
+			const int len = length_seen(p, l);
+			s_off[r] = len;                                // (the pages taken before are of no use here)
+			if (blockIdx.x == 0) {
+				p.row_start[r] = s_start[r];
+				p.lens[r] = len;
+				if (len < l.past + l.fresh) bad |= PAGED_NO_ROOM;
+			}
 		}
-		if (tid == 0) {
+		if (tid == 0 && blockIdx.x == 0) {
 			p.row_start[R] = used;
 			if (p.pool) *p.next_head = min(max(head, 0), p.pool_size) + min(taken, p.pool_size - min(max(head, 0), p.pool_size));
 		}
-		int *s_few = s_off + R + 1, *s_many = s_few + R + 1, *s_first = s_many + R + 1;
+		int *s_few = s_off + R + 1, *s_many = s_few + R + 1, *s_first = s_many + R + 1, *s_sorted = s_first + PL_KEEP;
+		PgEntry *s_entry = reinterpret_cast<PgEntry *>(pl_smem + (4 * (R + 1) + 2 * PL_KEEP + 3) / 4 * 4);
 		const int group = p.heads / p.kv_heads;
 		int few = 0, many = 0;
 		for (int base = 0; base < R; base += PL_THREADS) {
@@ -264,18 +295,18 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, 
 		}
 		__syncthreads();
 		const PgWork w = pg_work(p.work, R, p.rows, p.heads, p.kv_heads);
-		lay_out(p, 0, s_start, s_few, s_first, s_scan, w);
-		if (tiles) lay_out(p, 1, s_start, s_many, s_first, s_scan, w);
+		if (blockIdx.x < PL_PARTS) lay_out(p, 0, blockIdx.x, PL_PARTS, s_start, s_off, s_few, s_entry, s_first, s_sorted, s_scan, w);
+		else lay_out(p, 1, 0, 1, s_start, s_off, s_many, s_entry, s_first, s_sorted, s_scan, w);
 	} else {
 		// pages that are taken now: a warp per request
-		const int warps = (gridDim.x - 1) * (PL_THREADS / 32), lane = tid & 31;
+		const int others = gridDim.x - planners, me = blockIdx.x - planners, warps = others * (PL_THREADS / 32), lane = tid & 31;
 		if (p.pool)
-			for (int r = (blockIdx.x - 1) * (PL_THREADS / 32) + (tid >> 5); r < R; r += warps) {
+			for (int r = me * (PL_THREADS / 32) + (tid >> 5); r < R; r += warps) {
 				const Lengths l = lengths_of(p, r, bad);
 				if (l.full > p.table_width) bad |= PAGED_NO_ROOM;
 				for (int c = l.old + lane; c < min(l.full, p.table_width); c += 32) p.table[(int64_t)r * p.table_ld + c] = page_of(r, c, l.old);
 			}
-		for (int m = (blockIdx.x - 1) * PL_THREADS + tid; m < p.rows; m += (gridDim.x - 1) * PL_THREADS) {
+		for (int m = me * PL_THREADS + tid; m < p.rows; m += others * PL_THREADS) {
 			int pos = 0;
 			int64_t slot = -1;
 			if (m < used) {
@@ -299,9 +330,9 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, 
 
 int pg_plan_launch(const paged_plan_t &p, int dtype, cudaStream_t stream) {
 	const int tiles = p.pages > 0 && pg_tiles_serve(dtype, p.dim, p.page, p.max_fresh, p.heads, p.kv_heads);
-	const size_t smem = (size_t)(4 * (p.requests + 1) + PL_KEEP) * sizeof(int);
-	static_assert((4 * (PAGED_MAX_REQUESTS + 1) + PL_KEEP) * sizeof(int) + 4096 <= 227 * 1024, "shared memory");
-	const int fill = (int)((p.rows + (int64_t)PL_THREADS - 1) / PL_THREADS), ctas = 1 + (fill < 1 ? 1 : fill > 295 ? 295 : fill);
+	const size_t smem = (size_t)(4 * (p.requests + 1) + 2 * PL_KEEP + 3) * sizeof(int) + PL_NEAR * sizeof(PgEntry);
+	static_assert((4 * (PAGED_MAX_REQUESTS + 1) + 2 * PL_KEEP) * sizeof(int) + PL_NEAR * sizeof(PgEntry) + 6144 <= 227 * 1024, "shared memory");
+	const int fill = (int)((p.rows + (int64_t)PL_THREADS - 1) / PL_THREADS), ctas = PL_PARTS + (tiles ? 1 : 0) + (fill < 1 ? 1 : fill > 288 ? 288 : fill);
 	return pg_launch(plan_kernel, dim3(ctas), PL_THREADS, smem, stream, p, tiles);
 }
 
