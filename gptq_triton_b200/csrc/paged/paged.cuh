@@ -164,10 +164,9 @@ int pg_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cud
 int pg_plan_launch(const paged_plan_t &p, int dtype, cudaStream_t stream);
 int pg_append_launch(const paged_append_t &p, int dtype, cudaStream_t stream);
 int64_t pg_rows_scratch(const paged_attention_t &p);
-int pg_rows_launch(const paged_attention_t &p, int dtype, bool beside, cudaStream_t stream);          // fp16, bf16; beside: the tile kernel runs
+int pg_rows_launch(const paged_attention_t &p, int dtype, bool beside, cudaStream_t stream);          // beside: the tile kernel runs too
 int pg_join_launch(const paged_attention_t &p, int dtype, char *tile_scratch, cudaStream_t stream);          // of both kernels
 int64_t pg_tiles_scratch(const paged_attention_t &p);
 int pg_tiles_launch(const paged_attention_t &p, int dtype, char *scratch, cudaStream_t stream);
-int pg_attend_simple(const paged_attention_t &p, int dtype, cudaStream_t stream);
 
 }   // namespace gptq

@@ -71,7 +71,7 @@ int paged_append(const paged_append_t *p, int dtype, void *stream) {
 int64_t paged_attention_scratch(const paged_attention_t *p, int dtype) {
 	if (!p || !known(dtype) || p->dim < 1 || p->dim > PAGED_MAX_DIM) return -1;
 	if (!heads_ok(p->heads, p->kv_heads) || p->page < 1) return -1;
-	return dtype == PG_F32 ? 16 : pg_rows_scratch(*p) + (tiles(*p, dtype) ? pg_tiles_scratch(*p) : 0);
+	return pg_rows_scratch(*p) + (tiles(*p, dtype) ? pg_tiles_scratch(*p) : 0);
 }
 
 int paged_attention(const paged_attention_t *p, int dtype, void *stream) {
@@ -90,7 +90,6 @@ int paged_attention(const paged_attention_t *p, int dtype, void *stream) {
 	if (!steps_ok(p->k_page, p->k_kv, dtype) || !steps_ok(p->v_page, p->v_kv, dtype) || !steps_ok(p->q_row, p->q_head, dtype) || !aligned16(p->q) || !aligned16(p->k_cache) || !aligned16(p->v_cache) ||
 		!aligned16(p->out))
 		return GPTQ_ERR_ALIGN;
-	if (dtype == PG_F32) return pg_attend_simple(*p, dtype, (cudaStream_t)stream);
 	if (!p->scratch || !aligned16(p->scratch) || (int64_t)p->scratch_bytes < paged_attention_scratch(p, dtype)) return GPTQ_ERR_WORKSPACE;
 	const bool both = tiles(*p, dtype);
 	char *tile_scratch = both ? (char *)p->scratch + pg_rows_scratch(*p) : nullptr;

@@ -5,57 +5,6 @@ namespace gptq {
 
 namespace {
 
-// A warp serves one row and one query head: a lane holds entries lane, lane + 32 .. of the head; one key after the other with a running
-// maximum and sum.
-template <typename T>
-__global__ void __launch_bounds__(128) simple_kernel(const paged_attention_t p) {
-	pdl_wait();
-	pdl_trigger();
-	const int lane = threadIdx.x & 31;
-	const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-	const int m = (int)(at / p.heads), h = (int)(at % p.heads), kvh = h / (p.heads / p.kv_heads);
-	if (m >= p.rows || m >= p.row_start[p.requests]) return;
-	int lo = 0, hi = p.requests;
-	while (hi - lo > 1) {
-		const int mid = (lo + hi) >> 1;
-		if (p.row_start[mid] <= m) lo = mid;
-		else hi = mid;
-	}
-	const int r = lo, pos = p.lens[r] - (p.row_start[r + 1] - m);
-	constexpr int N = PAGED_MAX_DIM / 32;
-	float q[N], o[N], mx = -INFINITY, sum = 0.f;
-#pragma unroll
-	for (int i = 0; i < N; ++i) {
-		const int d = lane + 32 * i;
-		q[i] = d < p.dim ? PgElem<T>::get(reinterpret_cast<const T *>(p.q)[m * p.q_row + h * p.q_head + d]) * p.scale : 0.f;
-		o[i] = 0.f;
-	}
-	bool bad = false;
-	for (int j = 0; j <= pos; ++j) {
-		const int c = j / p.page;
-		const int id = c < p.table_width ? p.table[r * p.table_ld + c] : -1;
-		const bool there = id >= 0 && id < p.pages;
-		bad |= !there;
-		const T *k = reinterpret_cast<const T *>(p.k_cache) + id * p.k_page + kvh * p.k_kv + (int64_t)(j - c * p.page) * p.dim;
-		const T *v = reinterpret_cast<const T *>(p.v_cache) + id * p.v_page + kvh * p.v_kv + (int64_t)(j - c * p.page) * p.dim;
-		float s = 0.f;
-#pragma unroll
-		for (int i = 0; i < N; ++i)
-			if (there && lane + 32 * i < p.dim) s = fmaf(q[i], PgElem<T>::get(k[lane + 32 * i]), s);
-#pragma unroll
-		for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-		const float next = fmaxf(mx, s), keep = mx == -INFINITY ? 0.f : __expf(mx - next), w = __expf(s - next);
-		sum = sum * keep + w;
-#pragma unroll
-		for (int i = 0; i < N; ++i) o[i] = fmaf(w, there && lane + 32 * i < p.dim ? PgElem<T>::get(v[lane + 32 * i]) : 0.f, o[i] * keep);
-		mx = next;
-	}
-	if (bad && lane == 0) atomicOr(p.status, PAGED_BAD_INDEX);
-#pragma unroll
-	for (int i = 0; i < N; ++i)
-		if (lane + 32 * i < p.dim) reinterpret_cast<T *>(p.out)[((int64_t)m * p.heads + h) * p.dim + lane + 32 * i] = PgElem<T>::put(pos < 0 ? 0.f : o[i] / sum);
-}
-
 // ---- fp16 and bf16 ------------------------------------------------------------------------------------------------------------
 // Keys and values stream past up to 16 rows (new tokens times the query heads of a key head), which are the M of the MMAs whether or
 // not all of them are in use: S = Q K^T, weights, O += P V, fp32 sums, maximum and sum per row kept while the keys pass.  Bound by HBM: the
@@ -329,6 +278,210 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 	if (beside) pdl_wait();
 }
 
+// ---- fp32 ---------------------------------------------------------------------------------------------------------------------
+// The same walk without reduced-precision products.  Scores: a lane takes one of the 16 keys and half of the head's entries, the queries come
+// from shared memory; products with the values: a lane takes four entries of the head (or of every second key, for heads of 64), weights
+// come by shuffles.  ROWS: rows of a tile that the code provides for.
+template <int DP, int ROWS> struct FloatShape {
+	static constexpr int UNITS = DP / 4;
+	static constexpr int HALF = PG_KEYS * DP * 4;
+	static constexpr int STAGES = DP == 256 ? 1 : DP == 64 && ROWS > 4 ? 2 : 3;
+	static constexpr int Q_ROW = DP + 8;                             // the halves of a query 4 floats further apart: other banks
+	static constexpr int RING = RW_WARPS * STAGES * 2 * HALF;
+	static constexpr int SMEM = RING + RW_WARPS * ROWS * Q_ROW * 4;
+};
+
+template <int DP, int ROWS, bool EVEN>
+__global__ void __launch_bounds__(RW_THREADS, DP == 64 ? 2 : 1) rows_f32_kernel(const paged_attention_t p, const PgWork work) {
+	using S = FloatShape<DP, ROWS>;
+	extern __shared__ __align__(128) unsigned char rf_smem[];
+	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+	pdl_wait();
+	pdl_trigger();
+	const int slot = blockIdx.x * RW_WARPS + warp;
+	const PgEntry *entries = work.entries[0];
+	const int entry_count = read_list(work.list).entries;
+	const PgStart begin = read_start(work.starts[0] + slot), end = read_start(work.starts[0] + slot + 1);
+	Walk at;
+	if (!at.start(begin, end)) return;
+	Walk ahead = at;
+	const int group = p.heads / p.kv_heads;
+	const uint32_t ring = smem_u32(rf_smem) + warp * S::STAGES * 2 * S::HALF;
+	const float *ring_f = reinterpret_cast<const float *>(rf_smem + warp * S::STAGES * 2 * S::HALF);
+	float *s_q = reinterpret_cast<float *>(rf_smem + S::RING) + warp * ROWS * S::Q_ROW;
+	const float to_base2 = p.scale * PG_LOG2E;
+	int bad = 0, next_id = -1, next_row = 0;
+	bool more = true;
+	auto look_up = [&]() {
+		const int key = ahead.block * PG_KEYS + (EVEN ? 0 : lane & 15);
+		next_id = -1;
+		next_row = 0;
+		if (key < ahead.e.seen) {
+			const int c = key / p.page;
+			next_row = key - c * p.page;
+			next_id = c < p.table_width ? __ldcg(p.table + (int64_t)ahead.e.request * p.table_ld + c) : -2;
+		}
+	};
+	auto copy = [&](int stage) {
+		const bool there = next_id >= 0 && next_id < p.pages;
+		if (next_id != -1 && !there) bad = PAGED_BAD_INDEX;
+		const int left = ahead.e.seen - ahead.block * PG_KEYS;
+		// place of this lane's key (of the first one: EVEN) and of its values
+		const float *k = reinterpret_cast<const float *>(p.k_cache), *v = reinterpret_cast<const float *>(p.v_cache);
+		if (there) {
+			k += next_id * p.k_page + ahead.kv * p.k_kv + (int64_t)next_row * p.dim;
+			v += next_id * p.v_page + ahead.kv * p.v_kv + (int64_t)next_row * p.dim;
+		}
+		const uint32_t dst = ring + stage * 2 * S::HALF;
+#pragma unroll 4
+		for (int x = lane; x < PG_KEYS * S::UNITS; x += 32) {
+			const int row = x / S::UNITS, unit = x % S::UNITS;
+			unsigned long long kp = reinterpret_cast<unsigned long long>(k), vp = reinterpret_cast<unsigned long long>(v);
+			bool real = there;
+			if (EVEN) {
+				kp += (unsigned long long)row * p.dim * 4;
+				vp += (unsigned long long)row * p.dim * 4;
+				real = real && row < left;
+			} else {
+				kp = __shfl_sync(0xffffffffu, kp, row);
+				vp = __shfl_sync(0xffffffffu, vp, row);
+				real = __shfl_sync(0xffffffffu, (int)there, row);
+			}
+			real = real && 4 * unit < p.dim;
+			const uint32_t to = dst + row * DP * 4 + ((unit ^ (row & 7)) << 4);
+			cp_async16_or_zero(to, real ? reinterpret_cast<const void *>(kp + unit * 16) : p.k_cache, real ? 16 : 0);
+			cp_async16_or_zero(to + S::HALF, real ? reinterpret_cast<const void *>(vp + unit * 16) : p.v_cache, real ? 16 : 0);
+		}
+		more = ahead.step(end, entries, entry_count, p.kv_heads);
+		if (more) look_up();
+	};
+	look_up();
+#pragma unroll
+	for (int s = 0; s < S::STAGES; ++s) {
+		if (more) copy(s);
+		cp_async_commit();
+	}
+
+	constexpr int V4 = DP >= 128 ? DP / 128 : 1, SPLIT = DP >= 128 ? 1 : 2;          // float4 of a lane, lanes that share entries
+	float4 o[ROWS][V4];
+	float mx[ROWS], sum[ROWS];
+	int count = 0, least = 0, seen = 0, first_block = 0;      // seen: keys that row (lane & 15) sees
+	bool fresh = true;
+	const int key = lane & 15, side = lane >> 4;
+	for (int stage = 0;;) {
+		if (fresh) {
+			fresh = false;
+			first_block = at.block;
+			count = min(PG_ROWS, at.e.fresh * group - at.e.tile * PG_ROWS);
+			least = at.e.len - at.e.fresh + at.e.tile * PG_ROWS / group + 1;
+			const int mine = at.e.tile * PG_ROWS + key;
+			seen = key < count ? at.e.len - at.e.fresh + mine / group + 1 : 0;
+			__syncwarp();
+			for (int x = lane; x < ROWS * S::UNITS; x += 32) {
+				const int row = x / S::UNITS, d = x % S::UNITS * 4, token = (at.e.tile * PG_ROWS + row) / group, head = at.kv * group + (at.e.tile * PG_ROWS + row) - token * group;
+				float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+				if (row < count && d < p.dim) q = __ldcg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p.q) + (int64_t)(at.e.row + token) * p.q_row + (int64_t)head * p.q_head + d));
+				*reinterpret_cast<float4 *>(s_q + row * S::Q_ROW + d + (d >= DP / 2 ? 4 : 0)) = q;
+			}
+			__syncwarp();
+#pragma unroll
+			for (int r = 0; r < ROWS; ++r) {
+				mx[r] = -INFINITY;
+				sum[r] = 0.f;
+#pragma unroll
+				for (int i = 0; i < V4; ++i) o[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+			}
+		}
+		cp_async_wait<S::STAGES - 1>();
+		__syncwarp();
+		const float *sk = ring_f + stage * 2 * (S::HALF / 4), *sv = sk + S::HALF / 4;
+		const int key0 = at.block * PG_KEYS;
+		float w[ROWS];
+#pragma unroll
+		for (int r = 0; r < ROWS; ++r) w[r] = 0.f;
+#pragma unroll 4
+		for (int u = 0; u < DP / 8; ++u) {
+			const float4 k = *reinterpret_cast<const float4 *>(sk + key * DP + (((side * (DP / 8) + u) ^ (key & 7)) << 2));
+#pragma unroll
+			for (int r = 0; r < ROWS; ++r)
+				if (r < 4 || r < count) {
+					const float4 q = *reinterpret_cast<const float4 *>(s_q + r * S::Q_ROW + side * (DP / 2 + 4) + 4 * u);
+					w[r] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, w[r]))));
+				}
+		}
+		const bool edge = key0 + PG_KEYS > least;
+#pragma unroll
+		for (int r = 0; r < ROWS; ++r)
+			if (r < 4 || r < count) {
+				float s = (w[r] + __shfl_xor_sync(0xffffffffu, w[r], 16)) * to_base2;
+				if (edge && key0 + key >= __shfl_sync(0xffffffffu, seen, r)) s = -INFINITY;
+				float top = s;
+#pragma unroll
+				for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+				if (top > mx[r]) {                             // (the same in all lanes)
+					const float keep = mx[r] == -INFINITY ? 0.f : ex2(mx[r] - top);
+					mx[r] = top;
+					sum[r] *= keep;
+#pragma unroll
+					for (int i = 0; i < V4; ++i) o[r][i] = make_float4(o[r][i].x * keep, o[r][i].y * keep, o[r][i].z * keep, o[r][i].w * keep);
+				}
+				w[r] = ex2(s - (mx[r] == -INFINITY ? 0.f : mx[r]));
+				sum[r] += w[r];
+			}
+#pragma unroll 4
+		for (int j = 0; j < PG_KEYS / SPLIT; ++j) {
+			const int from = j * SPLIT + (SPLIT == 2 ? side : 0);
+			float4 v[V4];
+#pragma unroll
+			for (int i = 0; i < V4; ++i) v[i] = *reinterpret_cast<const float4 *>(sv + from * DP + (((lane % S::UNITS + 32 * i) ^ (from & 7)) << 2));
+#pragma unroll
+			for (int r = 0; r < ROWS; ++r)
+				if (r < 4 || r < count) {
+					const float x = __shfl_sync(0xffffffffu, w[r], from);
+#pragma unroll
+					for (int i = 0; i < V4; ++i) o[r][i] = make_float4(fmaf(x, v[i].x, o[r][i].x), fmaf(x, v[i].y, o[r][i].y), fmaf(x, v[i].z, o[r][i].z), fmaf(x, v[i].w, o[r][i].w));
+				}
+		}
+		__syncwarp();
+		if (more) copy(stage);
+		cp_async_commit();
+		stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+
+		const int blocks = at.e.blocks, last = at.block, entry_row = at.e.row, before = at.e.len - at.e.fresh, tile = at.e.tile, kv = at.kv;
+		const bool tile_ends = last + 1 == blocks, go_on = at.step(end, entries, entry_count, p.kv_heads);
+		if (!tile_ends && go_on) continue;
+		fresh = true;
+		const bool whole = first_block == 0 && tile_ends;
+		float *part = reinterpret_cast<float *>(p.scratch) + (int64_t)(2 * slot + (first_block == 0)) * PG_ROWS * (DP + 2);
+#pragma unroll
+		for (int r = 0; r < ROWS; ++r)
+			if (r < count) {
+#pragma unroll
+				for (int d = 8; d > 0; d >>= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], d);
+				const int token = (tile * PG_ROWS + r) / group, head = kv * group + tile * PG_ROWS + r - token * group;
+				const float f = !whole ? 1.f : before + token < 0 ? 0.f : 1.f / sum[r];
+				if (!whole && lane == 0) __stcg(reinterpret_cast<float2 *>(part + PG_ROWS * DP) + r, make_float2(mx[r], sum[r]));
+#pragma unroll
+				for (int i = 0; i < V4; ++i) {
+					float4 a = o[r][i];
+					if (SPLIT == 2) {
+						a.x += __shfl_xor_sync(0xffffffffu, a.x, 16);
+						a.y += __shfl_xor_sync(0xffffffffu, a.y, 16);
+						a.z += __shfl_xor_sync(0xffffffffu, a.z, 16);
+						a.w += __shfl_xor_sync(0xffffffffu, a.w, 16);
+					}
+					const int d = (lane % S::UNITS + 32 * i) * 4;
+					if (SPLIT == 2 && side) continue;
+					const float4 y = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
+					if (!whole) __stcg(reinterpret_cast<float4 *>(part + r * DP + d), y);
+					else if (d < p.dim) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.out) + ((int64_t)(entry_row + token) * p.heads + head) * p.dim + d) = y;
+				}
+			}
+		if (!go_on) break;
+	}
+	if (bad) atomicOr(p.status, bad);
+}
+
 int rows_dp(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 template <typename T, int DP>
@@ -348,19 +501,27 @@ int rows_launch_dim(const paged_attention_t &p, const PgWork &work, bool beside,
 	}
 }
 
+template <int DP, int ROWS>
+int rows_f32_launch_rows(const paged_attention_t &p, const PgWork &work, cudaStream_t stream) {
+	constexpr int smem = FloatShape<DP, ROWS>::SMEM;
+	static_assert(smem + 1024 <= (DP == 64 ? 114 : 228) * 1024 && smem <= 227 * 1024, "shared memory of an SM, 1 KB of it reserved per CTA");
+	if (p.page % PG_KEYS == 0) return pg_launch(rows_f32_kernel<DP, ROWS, true>, dim3(PG_SLOTS / RW_WARPS), RW_THREADS, smem, stream, p, work);
+	return pg_launch(rows_f32_kernel<DP, ROWS, false>, dim3(PG_SLOTS / RW_WARPS), RW_THREADS, smem, stream, p, work);
+}
+template <int DP>
+int rows_f32_launch(const paged_attention_t &p, const PgWork &work, cudaStream_t stream) {
+	const bool few = (int64_t)p.max_fresh * (p.heads / p.kv_heads) <= 4;
+	return few ? rows_f32_launch_rows<DP, 4>(p, work, stream) : rows_f32_launch_rows<DP, PG_ROWS>(p, work, stream);
+}
+
 }   // namespace
 
 int64_t pg_rows_scratch(const paged_attention_t &p) { return (int64_t)2 * PG_SLOTS * PG_ROWS * (rows_dp(p.dim) + 2) * 4; }
 
 int pg_rows_launch(const paged_attention_t &p, int dtype, bool beside, cudaStream_t stream) {
 	const PgWork work = pg_work(const_cast<int32_t *>(p.work), p.requests, p.rows, p.heads, p.kv_heads);
+	if (dtype == PG_F32) return p.dim <= 64 ? rows_f32_launch<64>(p, work, stream) : p.dim <= 128 ? rows_f32_launch<128>(p, work, stream) : rows_f32_launch<256>(p, work, stream);
 	return dtype == PG_BF16 ? rows_launch_dim<bf16>(p, work, beside, stream) : rows_launch_dim<__half>(p, work, beside, stream);
-}
-
-int pg_attend_simple(const paged_attention_t &p, int dtype, cudaStream_t stream) {
-	const unsigned ctas = (unsigned)(((int64_t)p.rows * p.heads + 3) / 4);
-	if (dtype == PG_F32) return pg_launch(simple_kernel<float>, dim3(ctas), 128, 0, stream, p);
-	return dtype == PG_BF16 ? pg_launch(simple_kernel<bf16>, dim3(ctas), 128, 0, stream, p) : pg_launch(simple_kernel<__half>, dim3(ctas), 128, 0, stream, p);
 }
 
 }   // namespace gptq
