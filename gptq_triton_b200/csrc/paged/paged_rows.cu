@@ -399,34 +399,53 @@ __global__ void __launch_bounds__(RW_THREADS, DP == 64 ? 2 : 1) rows_f32_kernel(
 		float w[ROWS];
 #pragma unroll
 		for (int r = 0; r < ROWS; ++r) w[r] = 0.f;
+		// (rows in groups of four, whose chains run side by side)
 #pragma unroll 4
 		for (int u = 0; u < DP / 8; ++u) {
 			const float4 k = *reinterpret_cast<const float4 *>(sk + key * DP + (((side * (DP / 8) + u) ^ (key & 7)) << 2));
 #pragma unroll
-			for (int r = 0; r < ROWS; ++r)
-				if (r < 4 || r < count) {
-					const float4 q = *reinterpret_cast<const float4 *>(s_q + r * S::Q_ROW + side * (DP / 2 + 4) + 4 * u);
-					w[r] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, w[r]))));
+			for (int g = 0; g < ROWS; g += 4)
+				if (g < count) {
+#pragma unroll
+					for (int r = g; r < g + 4; ++r) {
+						const float4 q = *reinterpret_cast<const float4 *>(s_q + r * S::Q_ROW + side * (DP / 2 + 4) + 4 * u);
+						w[r] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, w[r]))));
+					}
 				}
 		}
 		const bool edge = key0 + PG_KEYS > least;
 #pragma unroll
-		for (int r = 0; r < ROWS; ++r)
-			if (r < 4 || r < count) {
-				float s = (w[r] + __shfl_xor_sync(0xffffffffu, w[r], 16)) * to_base2;
-				if (edge && key0 + key >= __shfl_sync(0xffffffffu, seen, r)) s = -INFINITY;
-				float top = s;
+		for (int g = 0; g < ROWS; g += 4)
+			if (g < count) {
+				float top[4];
+				bool grown = false;
 #pragma unroll
-				for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-				if (top > mx[r]) {                             // (the same in all lanes)
-					const float keep = mx[r] == -INFINITY ? 0.f : ex2(mx[r] - top);
-					mx[r] = top;
-					sum[r] *= keep;
-#pragma unroll
-					for (int i = 0; i < V4; ++i) o[r][i] = make_float4(o[r][i].x * keep, o[r][i].y * keep, o[r][i].z * keep, o[r][i].w * keep);
+				for (int i = 0; i < 4; ++i) {
+					w[g + i] = (w[g + i] + __shfl_xor_sync(0xffffffffu, w[g + i], 16)) * to_base2;
+					if (edge && key0 + key >= __shfl_sync(0xffffffffu, seen, g + i)) w[g + i] = -INFINITY;
+					top[i] = w[g + i];
 				}
-				w[r] = ex2(s - (mx[r] == -INFINITY ? 0.f : mx[r]));
-				sum[r] += w[r];
+#pragma unroll
+				for (int d = 8; d > 0; d >>= 1)
+#pragma unroll
+					for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], d));
+#pragma unroll
+				for (int i = 0; i < 4; ++i) grown = grown || top[i] > mx[g + i];
+				if (grown) {                                   // (the same in all lanes)
+#pragma unroll
+					for (int i = 0; i < 4; ++i) {
+						const float next = fmaxf(mx[g + i], top[i]), keep = mx[g + i] == -INFINITY ? 0.f : ex2(mx[g + i] - next);
+						mx[g + i] = next;
+						sum[g + i] *= keep;
+#pragma unroll
+						for (int x = 0; x < V4; ++x) o[g + i][x] = make_float4(o[g + i][x].x * keep, o[g + i][x].y * keep, o[g + i][x].z * keep, o[g + i][x].w * keep);
+					}
+				}
+#pragma unroll
+				for (int i = 0; i < 4; ++i) {
+					w[g + i] = ex2(w[g + i] - (mx[g + i] == -INFINITY ? 0.f : mx[g + i]));
+					sum[g + i] += w[g + i];
+				}
 			}
 #pragma unroll 4
 		for (int j = 0; j < PG_KEYS / SPLIT; ++j) {
@@ -435,11 +454,14 @@ __global__ void __launch_bounds__(RW_THREADS, DP == 64 ? 2 : 1) rows_f32_kernel(
 #pragma unroll
 			for (int i = 0; i < V4; ++i) v[i] = *reinterpret_cast<const float4 *>(sv + from * DP + (((lane % S::UNITS + 32 * i) ^ (from & 7)) << 2));
 #pragma unroll
-			for (int r = 0; r < ROWS; ++r)
-				if (r < 4 || r < count) {
-					const float x = __shfl_sync(0xffffffffu, w[r], from);
+			for (int g = 0; g < ROWS; g += 4)
+				if (g < count) {
 #pragma unroll
-					for (int i = 0; i < V4; ++i) o[r][i] = make_float4(fmaf(x, v[i].x, o[r][i].x), fmaf(x, v[i].y, o[r][i].y), fmaf(x, v[i].z, o[r][i].z), fmaf(x, v[i].w, o[r][i].w));
+					for (int r = g; r < g + 4; ++r) {
+						const float x = __shfl_sync(0xffffffffu, w[r], from);
+#pragma unroll
+						for (int i = 0; i < V4; ++i) o[r][i] = make_float4(fmaf(x, v[i].x, o[r][i].x), fmaf(x, v[i].y, o[r][i].y), fmaf(x, v[i].z, o[r][i].z), fmaf(x, v[i].w, o[r][i].w));
+					}
 				}
 		}
 		__syncwarp();
