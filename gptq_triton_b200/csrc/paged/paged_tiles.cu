@@ -241,83 +241,64 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 		__syncwarp();
 	}
 	if (warp == TL_MMA) {
-		constexpr uint32_t base = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(TL_SIDE >> 4) << 24);          // D fp32, M = 128
-		constexpr uint32_t id_qk = base | ((uint32_t)(TL_KEYS >> 3) << 17), id_pv = base | (1u << 16) | ((uint32_t)(DP >> 3) << 17);      // values: N contiguous
-		const bool one = elect();
-		int n = 0;                                         // blocks of the ring consumed
-		uint32_t nq = 0, np[2] = {0, 0};
-		bool ok = true;
-		auto wait = [&](uint32_t bar, uint32_t parity) {
-			ok = ok && wait_fast(bar, parity & 1, stop);
-			if (!__all_sync(0xffffffffu, ok)) {
-				ok = false;
-				fail();
-			}
-			tc_fence_after();
-			return ok;
-		};
-		auto full = [&](int i) { return wait(bar_full + 8 * (i % S::RING), i / S::RING); };
-		auto qk = [&](int s, int i) {
-			if (one) {
+		if (elect()) {
+			constexpr uint32_t base = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(TL_SIDE >> 4) << 24);          // D fp32, M = 128
+			constexpr uint32_t id_qk = base | ((uint32_t)(TL_KEYS >> 3) << 17), id_pv = base | (1u << 16) | ((uint32_t)(DP >> 3) << 17);      // values: N contiguous
+			int n = 0;                                     // blocks of the ring consumed
+			uint32_t nq = 0, np[2] = {0, 0};
+			bool ok = true;
+			auto wait = [&](uint32_t bar, uint32_t parity) {
+				if (ok && !wait_fast(bar, parity & 1, stop)) {
+					ok = false;
+					fail();
+				}
+				return ok;
+			};
+			auto full = [&](int i) { return wait(bar_full + 8 * (i % S::RING), i / S::RING); };
+			auto qk = [&](int s, int i) {
 				const uint64_t qd = smem_desc_sw128(sq + s * S::BLOCK), kd = smem_desc_sw128(ring + (i % S::RING) * S::BLOCK);
 #pragma unroll
 				for (int k = 0; k < DP / 16; ++k) umma_f16(tmem + s * TL_KEYS, qd + (k >> 2) * (TL_CHUNK / 16) + 2 * (k & 3), kd + (k >> 2) * (TL_CHUNK / 16) + 2 * (k & 3), id_qk, k ? 1u : 0u);
 				umma_commit(bar_s + 8 * s);
-			}
-			__syncwarp();
-		};
-		auto pv = [&](int s, int i, int half, bool first) {          // 64 of the 128 keys
-			if (one) {
+			};
+			auto pv = [&](int s, int i, int half, bool first) {          // 64 of the 128 keys
 				const uint64_t vd = desc_values(ring + (i % S::RING) * S::BLOCK);
+				tc_fence_after();
 #pragma unroll
 				for (int k = half * (TL_KEYS / 32); k < (half + 1) * (TL_KEYS / 32); ++k) umma_f16_ts(tmem + S::O_AT + s * DP, tmem + s * TL_KEYS + 8 * k, vd + 128 * k, id_pv, first && k == 0 ? 0u : 1u);
-			}
-			__syncwarp();
-		};
-		auto commit = [&](uint32_t bar) {
-			if (one) umma_commit(bar);
-			__syncwarp();
-		};
-		for (; have && ok; have = it.next(), ++nq) {
-			// side s: blocks it.j0 .. ends[s] - 1
-			const int ends[2] = {min(it.j1, side_blocks(it.e, 0, group)), min(it.j1, side_blocks(it.e, 1, group))};
-			if (!full(n)) break;
-			for (int s = 0; s < 2 && ok; ++s) {
-				if (!wait(bar_q + 8 * s, nq)) break;
-				if (it.j0 < ends[s]) qk(s, n);
-				else commit(bar_none + 8 * s);
-			}
-			if (!ok) break;
-			commit(bar_free + 8 * (n % S::RING));
-			for (int j = it.j0; j < it.j1 && ok; ++j, n += 2) {
-				if (!full(n + 1)) break;
-				const int tail = it.e.seen - j * TL_KEYS;
-				if (tail < TL_KEYS) {                      // (only the last block of a tile)
-					const uint32_t v = ring + ((n + 1) % S::RING) * S::BLOCK;
-					for (int x = lane; x < (TL_KEYS - tail) * 8 * S::CHUNKS; x += 32) {
-						const int unit = x & 7, rest = x >> 3, c = rest % S::CHUNKS, r = tail + rest / S::CHUNKS;
-						asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + c * TL_CHUNK + r * 128 + unit * 16), "r"(0) : "memory");
-					}
-					fence_proxy_async();
-					__syncwarp();
-				}
-				const bool again = j + 1 < it.j1;
-				if (again && !full(n + 2)) break;
-				for (int s = 0; s < 2 && ok; ++s) {
-					if (j < ends[s]) {
-						if (wait(bar_p + 8 * s, np[s])) pv(s, n + 1, 0, j == it.j0);
-						if (wait(bar_p2 + 8 * s, np[s]++)) pv(s, n + 1, 1, false);
-					}
-					if (ok && j + 1 < ends[s]) qk(s, n + 2);
-					if (ok && j + 1 == ends[s]) commit(bar_o + 8 * s);
+			};
+			for (; have && ok; have = it.next(), ++nq) {
+				// side s: blocks it.j0 .. ends[s] - 1
+				const int ends[2] = {min(it.j1, side_blocks(it.e, 0, group)), min(it.j1, side_blocks(it.e, 1, group))};
+				if (!full(n)) break;
+				for (int s = 0; s < 2; ++s) {
+					if (!wait(bar_q + 8 * s, nq)) break;
+					tc_fence_after();
+					if (it.j0 < ends[s]) qk(s, n);
+					else umma_commit(bar_none + 8 * s);
 				}
 				if (!ok) break;
-				commit(bar_free + 8 * ((n + 1) % S::RING));
-				if (again) commit(bar_free + 8 * ((n + 2) % S::RING));
+				umma_commit(bar_free + 8 * (n % S::RING));
+				for (int j = it.j0; j < it.j1; ++j, n += 2) {
+					const bool again = j + 1 < it.j1;
+					if (!full(n + 1) || (again && !full(n + 2))) break;
+					for (int s = 0; s < 2 && ok; ++s) {
+						if (j < ends[s]) {
+							if (wait(bar_p + 8 * s, np[s])) pv(s, n + 1, 0, j == it.j0);
+							if (wait(bar_p2 + 8 * s, np[s]++)) pv(s, n + 1, 1, false);
+						}
+						if (ok && j + 1 < ends[s]) qk(s, n + 2);
+						if (ok && j + 1 == ends[s]) umma_commit(bar_o + 8 * s);
+					}
+					if (!ok) break;
+					umma_commit(bar_free + 8 * ((n + 1) % S::RING));
+					if (again) umma_commit(bar_free + 8 * ((n + 2) % S::RING));
+				}
+				if (!ok) break;
 			}
+			umma_commit(bar_end);                          // every MMA has completed before tensor memory goes back
+			mbar_wait_bounded(bar_end, 0, TL_SPIN);
 		}
-		commit(bar_end);                                 // every MMA has completed before tensor memory goes back
-		mbar_wait_bounded(bar_end, 0, TL_SPIN);
 		__syncwarp();
 	}
 	} else {
@@ -328,6 +309,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 		constexpr float LIFT = F16 ? 7.f : 0.f;            // fp16 weights up to 2^15: small ones stay above its subnormal range
 		const bool sectors = p.dim % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;          // rows in whole sectors of 32 bytes
 		uint32_t ns = 0, no = 0, nn = 0;
+		int blocks = 0;                                    // of the ring before this tile's
 		bool ok = true;
 		auto wait = [&](uint32_t bar, uint32_t parity) {
 			ok = ok && wait_fast(bar, parity & 1, stop);
@@ -421,6 +403,18 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 						w[k] = pack2<T>(a, b);
 					}
 					tmem_st32(ts + 32 * h, w);
+					if (h == 0 && it.e.seen - j * TL_KEYS < TL_KEYS) {
+						// The last block of a tile: values behind the last key seen become zeros before the weights are handed over (both sides write
+						// the same, each before its own products).
+						const int i = blocks + 2 * (j - it.j0) + 1, tail = it.e.seen - j * TL_KEYS;
+						wait(bar_full + 8 * (i % S::RING), i / S::RING);
+						const uint32_t v = ring + (i % S::RING) * S::BLOCK;
+						for (int x = tid & (TL_SIDE - 1); x < (TL_KEYS - tail) * 8 * S::CHUNKS; x += TL_SIDE) {
+							const int unit = x & 7, rest = x >> 3, c = rest % S::CHUNKS, r = tail + rest / S::CHUNKS;
+							asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + c * TL_CHUNK + r * 128 + unit * 16), "r"(0) : "memory");
+						}
+						fence_proxy_async();
+					}
 					tmem_st_wait();
 					tc_fence_before();
 					mbar_arrive((h ? bar_p2 : bar_p) + 8 * side);
@@ -429,6 +423,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 			if (!ok) break;
 			// the next tile's queries go first: its scores are computed while this one's results are stored
 			const PgEntry e = it.e;
+			blocks += 2 * (it.j1 - it.j0);
 			const int kv = it.kv, j0 = it.j0, j1 = it.j1, my_token = token, my_head = head, my_sees = sees;
 			// A side without blocks in this tile must not run ahead of the MMA warp: a wait tells a phase from its neighbours only.  (Not bar_o:
 			// the MMA warp may come to this while the results of the tile before still wait to be read.)
