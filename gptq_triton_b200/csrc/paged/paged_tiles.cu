@@ -164,10 +164,10 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 			mbar_init(bar_free + 8 * i, 1);
 		}
 		for (int i = 0; i < 2; ++i) {
-			mbar_init(bar_q + 8 * i, TL_SIDE);
+			mbar_init(bar_q + 8 * i, TL_SIDE / 32);          // a lane per warp arrives: 128 arrivals at one barrier take longer than the wait for them
 			mbar_init(bar_s + 8 * i, 1);
-			mbar_init(bar_p + 8 * i, TL_SIDE);
-			mbar_init(bar_p2 + 8 * i, TL_SIDE);
+			mbar_init(bar_p + 8 * i, TL_SIDE / 32);
+			mbar_init(bar_p2 + 8 * i, TL_SIDE / 32);
 			mbar_init(bar_o + 8 * i, 1);
 			mbar_init(bar_none + 8 * i, 1);
 		}
@@ -338,7 +338,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 			cp_async_commit();
 			cp_async_wait<0>();
 			fence_proxy_async();
-			mbar_arrive(bar_q + 8 * side);
+			__syncwarp();
+			if (lane == 0) mbar_arrive(bar_q + 8 * side);
 		};
 		queries();
 		while (have && ok) {
@@ -389,6 +390,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 				}
 				const float at = ref == -INFINITY ? 0.f : LIFT - ref;
 				const f32x2 mul = pair(scale2, scale2), off = pair(at, at);
+				f32x2 sums[4] = {total, pair(0.f, 0.f), pair(0.f, 0.f), pair(0.f, 0.f)};          // four chains of additions
 #pragma unroll
 				for (int h = 0; h < 2; ++h) {
 					uint32_t w[32];
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 						parts(fma2(pair(s[c][i], s[c][i + 1]), mul, off), a, b);
 						a = ex2(a);
 						b = ex2(b);
-						total = add2(total, pair(a, b));
+						sums[k & 3] = add2(sums[k & 3], pair(a, b));
 						w[k] = pack2<T>(a, b);
 					}
 					tmem_st32(ts + 32 * h, w);
@@ -417,8 +419,10 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 					}
 					tmem_st_wait();
 					tc_fence_before();
-					mbar_arrive((h ? bar_p2 : bar_p) + 8 * side);
+					__syncwarp();
+					if (lane == 0) mbar_arrive((h ? bar_p2 : bar_p) + 8 * side);
 				}
+				total = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
 			}
 			if (!ok) break;
 			// the next tile's queries go first: its scores are computed while this one's results are stored
