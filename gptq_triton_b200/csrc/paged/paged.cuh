@@ -38,6 +38,10 @@ template <> struct PgElem<__half> {
 // into equal lengths for the slots (warps of one kernel, CTAs of the other): whatever the lengths of the requests, no slot has more to
 // do than another.  A cut inside a job leaves partial results, which are joined; slot c works from starts[c] to starts[c + 1].
 constexpr int PG_ROWS = 16, PG_KEYS = 16, PG_SLOTS = 1184;
+// Requests of up to so many rows per key head go to the kernel for few rows.  us, few rows / tiles: 16 requests behind 300 to 5 000 tokens, 32 heads
+// over 8, 20 rows 51 / 57, 32 rows 57 / 60, 40 rows 71 / 61, heads of 64 38 / 43, 43 / 43, 54 / 43; one request behind 3 000 25 / 31, 25 / 34, 25 / 34.  A key
+// head of its own for every head is another matter, there is twice the cache to read for two tiles: 20 rows 166 / 150, 32 rows 176 / 119.
+inline __host__ __device__ int pg_few(int group) { return group > 1 ? 32 : PG_ROWS; }
 constexpr int PG_TILE = 256, PG_TILE_KEYS = 128, PG_TILE_SLOTS = 148;
 inline __host__ __device__ int pg_begin(int kind) { return kind ? 2 : 1; }
 
@@ -45,6 +49,7 @@ struct PgList {                        // of one of the two kernels; behind it i
 	int entries;
 	int whole;                          // slots take whole jobs by `order` instead (tile kernel)
 	int64_t per, total;                 // length of a slot's share, of all jobs
+	int cuts[2];                        // slots in which a job begins that ends in a later one: how many, in the two parts of the list
 };
 struct alignas(16) PgEntry {
 	int request, tile, blocks, first;   // blocks of keys that the tile sees; length of the entries before, per key head
@@ -61,7 +66,8 @@ struct alignas(16) PgStart {                       // entry -1: behind the last 
 __device__ __forceinline__ PgList read_list(const PgList *p) {
 	const int2 a = __ldcg(reinterpret_cast<const int2 *>(p));
 	const long long b = __ldcg(reinterpret_cast<const long long *>(p) + 1), c = __ldcg(reinterpret_cast<const long long *>(p) + 2);
-	return PgList{a.x, a.y, b, c};
+	const int2 d = __ldcg(reinterpret_cast<const int2 *>(p) + 3);
+	return PgList{a.x, a.y, b, c, {d.x, d.y}};
 }
 __device__ __forceinline__ PgStart read_start(const PgStart *p) {
 	const int4 a = __ldcg(reinterpret_cast<const int4 *>(p)), b = __ldcg(reinterpret_cast<const int4 *>(p) + 1), c = __ldcg(reinterpret_cast<const int4 *>(p) + 2);
@@ -77,6 +83,7 @@ struct PgWork {
 	PgStart *starts[2];                 // [slots + 1]
 	PgEntry *entries[2];
 	int *order;
+	int *cuts[2];                       // [2 PG_SLOTS], [2 PG_TILE_SLOTS]: the slots of both parts
 	int cap[2];
 	int64_t ints;
 };
@@ -96,12 +103,16 @@ inline __host__ __device__ PgWork pg_work(int32_t *base, int requests, int rows,
 	w.entries[1] = reinterpret_cast<PgEntry *>(base + at);
 	at += 8 * (int64_t)w.cap[1];
 	w.order = base + at;
-	w.ints = at + w.cap[1];
+	at += w.cap[1];
+	w.cuts[0] = base + at;
+	at += 2 * PG_SLOTS;
+	w.cuts[1] = base + at;
+	w.ints = at + 2 * PG_TILE_SLOTS;
 	return w;
 }
 // Whether the tensor-core kernel serves these sizes; which requests it then takes (more rows than PG_ROWS) is decided on the device.
 inline bool pg_tiles_serve(int dtype, int dim, int page, int max_fresh, int heads, int kv_heads) {
-	return dtype != PG_F32 && dim <= 128 && dim % 8 == 0 && (page == 8 || page == 16 || page == 32 || page == 64 || page % PG_TILE_KEYS == 0) && (int64_t)max_fresh * (heads / kv_heads) > PG_ROWS;
+	return dtype != PG_F32 && dim <= 128 && dim % 8 == 0 && (page == 8 || page == 16 || page == 32 || page == 64 || page % PG_TILE_KEYS == 0) && (int64_t)max_fresh * (heads / kv_heads) > pg_few(heads / kv_heads);
 }
 
 // cp.async of 16 bytes; `bytes` 0 writes zeros and reads nothing

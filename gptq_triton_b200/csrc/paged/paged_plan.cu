@@ -175,12 +175,20 @@ __device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, co
 		__syncthreads();
 		whole = s_span <= per + PL_JOIN;
 	}
-	if (tid == 0 && part == 0) w.list[kind] = PgList{E, whole, per, total};
+	if (tid == 0 && part == 0) {
+		int4 *dst = reinterpret_cast<int4 *>(w.list + kind);          // (the counts of cuts follow)
+		dst[0] = make_int4(E, whole, (int)(per & 0xffffffff), (int)(per >> 32));
+		reinterpret_cast<int2 *>(dst)[2] = make_int2((int)(total & 0xffffffff), (int)(total >> 32));
+		if (whole || parts == 1) w.list[kind].cuts[1] = 0;
+		if (whole) w.list[kind].cuts[0] = 0;
+	}
 	if (whole) return;                                     // (nobody looks at the starts)
-	for (int c = part * PL_THREADS + tid; c <= slots; c += parts * PL_THREADS) {
+	int cuts = 0;
+	for (int base = part * PL_THREADS; base <= slots; base += parts * PL_THREADS) {
+		const int c = base + tid;
 		const int64_t u = c * per;
 		PgStart s = {-1, 0, 0, 0, {}};
-		if (u < total) {
+		if (c <= slots && u < total) {
 			const bool small = total < PL_LIMIT;
 			const int x = small ? (int)u / p.kv_heads : (int)(u / p.kv_heads);
 			int e;
@@ -202,11 +210,20 @@ __device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, co
 			s.kv = small ? (int)rest / n : (int)(rest / n);
 			s.block = max((int)(rest - (int64_t)s.kv * n) - pg_begin(kind), 0);
 		}
-		int4 *dst = reinterpret_cast<int4 *>(w.starts[kind] + c);          // (16 bytes at a time: word by word these stores take half of the kernel's time)
-		dst[0] = make_int4(s.entry, s.kv, s.block, 0);
-		dst[1] = make_int4(s.job.request, s.job.tile, s.job.blocks, s.job.first);
-		dst[2] = make_int4(s.job.row, s.job.fresh, s.job.len, s.job.seen);
+		if (c <= slots) {
+			int4 *dst = reinterpret_cast<int4 *>(w.starts[kind] + c);          // (16 bytes at a time: word by word these stores take half of the kernel's time)
+			dst[0] = make_int4(s.entry, s.kv, s.block, 0);
+			dst[1] = make_int4(s.job.request, s.job.tile, s.job.blocks, s.job.first);
+			dst[2] = make_int4(s.job.row, s.job.fresh, s.job.len, s.job.seen);
+		}
+		// the first cut of a job lies less than a share behind its begin
+		int at = s.entry >= 0 && s.block > 0 && s.block <= per, none = 0, count, unused;
+		const bool cut = at;
+		scan2(at, none, PL_LIMIT, PL_LIMIT, count, unused, s_scan);
+		if (cut) w.cuts[kind][part * slots + cuts + at] = c - 1;
+		cuts += count;
 	}
+	if (tid == 0) w.list[kind].cuts[part] = cuts;
 }
 
 __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, int tiles) {
@@ -277,7 +294,7 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, 
 			int a = 0, b = 0;
 			if (r < R) {
 				const int64_t n = (int64_t)(s_start[r + 1] - s_start[r]) * group;
-				if (tiles && n > PG_ROWS) b = (int)((n + PG_TILE - 1) / PG_TILE);
+				if (tiles && n > pg_few(group)) b = (int)((n + PG_TILE - 1) / PG_TILE);
 				else a = (int)((n + PG_ROWS - 1) / PG_ROWS);
 			}
 			int ta, tb;

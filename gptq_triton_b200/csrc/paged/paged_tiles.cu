@@ -204,6 +204,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 		const int sub = lane / S::CHUNKS, chunk = lane % S::CHUNKS;
 		int n = 0, bad = 0;
 		bool ok = true;
+		const bool one = elect();
 		for (; have && ok; have = it.next()) {
 			const int *row = p.table + (int64_t)it.e.request * p.table_ld;
 			auto page_at = [&](int j) {                    // page and row in it of this lane's part of block j
@@ -231,7 +232,13 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 					}
 					if (lane == 0) mbar_arrive_expect_tx(bar_full + 8 * b, S::BLOCK);
 					__syncwarp();
-					if (lane < loads) tma_load_4d(ring + b * S::BLOCK + chunk * TL_CHUNK + sub * box * 128, v ? &tmv : &tmk, 64 * chunk, r0, it.kv, now, bar_full + 8 * b);
+					for (int x = 0; x < per_block; ++x) {
+						const int page = __shfl_sync(0xffffffffu, now, x * S::CHUNKS), first = __shfl_sync(0xffffffffu, r0, x * S::CHUNKS);
+						if (one) {
+#pragma unroll
+							for (int c = 0; c < S::CHUNKS; ++c) tma_load_4d(ring + b * S::BLOCK + c * TL_CHUNK + x * box * 128, v ? &tmv : &tmk, 64 * c, first, it.kv, page, bar_full + 8 * b);
+						}
+					}
 				}
 			}
 		}
