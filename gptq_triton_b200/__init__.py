@@ -11,7 +11,8 @@ from .lifinex import LifinexConfig, LifinexEngine, LifinexForCausalLM, load_lifi
 from .llama import DecodeEngine, LlamaConfig, LlamaForCausalLM
 from .loader import autotune_warmup, load_quant, save_quant, synthetic_quantized_llama
 from .paged import PagedPlan, paged_append, paged_attention, paged_plan
-from .registry import ARCHITECTURES, load_model, make_engine
+from .paged_engine import PagedEngine
+from .registry import ARCHITECTURES, load_model, make_engine, make_paged_engine
 from .quant_linear import QuantLinear, dequantize, make_quant, qmatmul, triton_matmul4, unpack_qweight, unpack_qzeros
 
 __all__ = [
@@ -22,7 +23,7 @@ __all__ = [
 	'load_model', 'make_engine', 'ARCHITECTURES',
 	'BefalixConfig', 'BefalixEngine', 'BefalixForCausalLM', 'load_befalix', 'synthetic_befalix',
 	'LifinexConfig', 'LifinexEngine', 'LifinexForCausalLM', 'load_lifinex', 'synthetic_lifinex',
-	'PagedPlan', 'paged_plan', 'paged_append', 'paged_attention',
+	'PagedPlan', 'paged_plan', 'paged_append', 'paged_attention', 'PagedEngine', 'make_paged_engine',
 	'dequantize', 'unpack_qweight', 'unpack_qzeros',
 	'quant_linear', 'fused_mlp',
 ]

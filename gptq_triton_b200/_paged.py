@@ -1,18 +1,16 @@
-"""ctypes binding of libpaged_b200.so (declared in include/paged_b200.h).  Like the other bindings it has no fallback: a missing
-library or a failing kernel raises."""
+"""ctypes binding of the paged-cache entry points of libgptq_b200.so (declared in include/paged_b200.h).  Like the other bindings it has
+no fallback: a missing library or a failing kernel raises."""
 from __future__ import annotations
 
 import ctypes
 import threading
 from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p
-from pathlib import Path
 from typing import Dict, Optional
 
 import torch
 
-from ._lib import GptqB200Error, ptr, register_status_buffer, require_cuda, stream_ptr      # noqa: F401
+from ._lib import LIB_PATH, GptqB200Error, ptr, register_status_buffer, require_cuda, stream_ptr      # noqa: F401
 
-LIB_PATH = Path(__file__).resolve().parent / 'libpaged_b200.so'
 CONTROL_BYTES = 16384
 MAX_REQUESTS = 8192
 MAX_DIM = 256

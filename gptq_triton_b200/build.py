@@ -1,11 +1,11 @@
 """Builds the in-tree C-ABI libraries with the sm_100a kernels with nvcc, and the extension module that calls them from Python:
 
-  libgptq_b200.so    4-bit quantised linear layers, attention and decode kernels   (csrc/*.cu)
+  libgptq_b200.so    4-bit quantised linear layers, attention and decode kernels   (csrc/*.cu),
+                     cache in pages                                                (csrc/paged/*.cu)
   libdense_b200.so   dense-weight layers and latent attention                      (csrc/dense/*.cu)
-  libpaged_b200.so   block tables, rows and attention of a cache in pages          (csrc/paged/*.cu)
   _host.so           layer calls without ctypes, against torch's C++ library       (csrc/host/*.cpp, with g++)
 
-Usage:  python -m gptq_triton_b200.build [--force] [--verbose] [gptq] [dense] [paged] [host]
+Usage:  python -m gptq_triton_b200.build [--force] [--verbose] [gptq] [dense] [host]
 """
 from __future__ import annotations
 
@@ -24,14 +24,12 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / 'csrc'
 LIB = PKG / 'libgptq_b200.so'
 DENSE_LIB = PKG / 'libdense_b200.so'
-PAGED_LIB = PKG / 'libpaged_b200.so'
 HOST_LIB = PKG / '_host.so'
 
-# library -> (output, folder of its sources, further folders whose headers they include)
+# library -> (output, folder of its sources, further folders whose headers they include; gptq: whose sources belong to it, too)
 TARGETS = {
-	'gptq': (LIB, CSRC, []),
+	'gptq': (LIB, CSRC, [CSRC / 'paged']),
 	'dense': (DENSE_LIB, CSRC / 'dense', [CSRC]),
-	'paged': (PAGED_LIB, CSRC / 'paged', [CSRC]),
 	'host': (HOST_LIB, CSRC / 'host', []),
 }
 
@@ -49,7 +47,9 @@ def _nvcc() -> str:
 
 
 def sources(target: str = 'gptq'):
-	return sorted(TARGETS[target][1].glob('*.cpp' if target == 'host' else '*.cu'))
+	_, folder, more = TARGETS[target]
+	files = sorted(folder.glob('*.cpp' if target == 'host' else '*.cu'))
+	return files + sorted(f for d in more for f in d.glob('*.cu')) if target == 'gptq' else files
 
 
 def _host_command(out: str):

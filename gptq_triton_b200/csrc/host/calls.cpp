@@ -373,7 +373,7 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
 	return none();
 }
 
-// ---- cache in pages (libpaged_b200.so) ---------------------------------------------------------------------------------------
+// ---- cache in pages ---------------------------------------------------------------------------------------
 decltype(&paged_plan) plan_fn = nullptr;
 decltype(&paged_append) append_fn = nullptr;
 decltype(&paged_attention) attention_fn = nullptr;

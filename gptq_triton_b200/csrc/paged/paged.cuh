@@ -1,4 +1,4 @@
-// Shared pieces of the paged-cache library: argument blocks, element access, the layout of the attention's work lists.
+// Shared pieces of the paged cache: argument blocks, element access, the layout of the attention's work lists.
 #pragma once
 
 #include <atomic>
@@ -152,7 +152,7 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 	asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
-// Launch with programmatic stream serialisation: every kernel of this library touches nothing that an earlier one wrote, and writes
+// Launch with programmatic stream serialisation: every kernel here touches nothing that an earlier one wrote, and writes
 // nothing, before its pdl_wait(), and triggers its successor behind it.  (The kernel for few rows is the exception, see there.)
 int pg_smem_opt_in(const void *kernel);
 template <typename... KArgs, typename... Args>

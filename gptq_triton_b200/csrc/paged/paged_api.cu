@@ -1,9 +1,7 @@
-// C ABI of the paged-cache library: checks of arguments and the choice of kernels.
+// C ABI of the paged cache: checks of arguments and the choice of kernels.
 #include "paged.cuh"
 
 namespace gptq {
-thread_local int g_last_cuda_error = 0;
-
 // All the shared memory that a kernel may have, asked for once per kernel and device.
 int pg_smem_opt_in(const void *kernel) {
 	static std::atomic<const void *> kernels[32];

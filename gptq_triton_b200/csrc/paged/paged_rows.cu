@@ -82,7 +82,8 @@ __global__ void __launch_bounds__(RW_THREADS, DP <= 128 ? 2 : 1) rows_kernel(con
 		if (key < ahead.e.seen) {
 			const int c = key / p.page;
 			next_row = key - c * p.page;
-			next_id = c < p.table_width ? __ldcg(p.table + (int64_t)ahead.e.request * p.table_ld + c) : -2;
+			next_id = c < p.table_width ? max(__ldcg(p.table + (int64_t)ahead.e.request * p.table_ld + c), -1) : -1;
+			if (next_id < 0) next_id = -2;                 // a key without a page
 		}
 	};
 	auto copy = [&](int stage) {
@@ -319,7 +320,8 @@ __global__ void __launch_bounds__(RW_THREADS, DP == 64 ? 2 : 1) rows_f32_kernel(
 		if (key < ahead.e.seen) {
 			const int c = key / p.page;
 			next_row = key - c * p.page;
-			next_id = c < p.table_width ? __ldcg(p.table + (int64_t)ahead.e.request * p.table_ld + c) : -2;
+			next_id = c < p.table_width ? max(__ldcg(p.table + (int64_t)ahead.e.request * p.table_ld + c), -1) : -1;
+			if (next_id < 0) next_id = -2;                 // a key without a page
 		}
 	};
 	auto copy = [&](int stage) {

@@ -1,0 +1,258 @@
+"""Serving of LLaMA models from a cache in pages: requests of different lengths side by side, prompts in portions beside decode steps,
+pages given back when a request ends.
+
+	engine = PagedEngine(model, pages=4096)
+	a = engine.add([1, 2, 3], steps=20)          # a request: prompt, tokens to generate
+	while engine.busy:
+		for request, token in engine.step():      # one step of all requests that run
+			...
+or engine.generate(prompts, steps).  Decoding is greedy.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass, field
+from typing import Dict, List, Optional, Sequence, Tuple
+
+import torch
+
+from .fused_attention import QuantLlamaAttention
+from .fused_attention import rmsnorm as rmsnorm_kernel
+from ._paged import MAX_REQUESTS
+from .paged import paged_append, paged_attention, paged_plan
+
+
+@dataclass
+class _Request:
+	number: int
+	prompt: List[int]
+	steps: int
+	stop: Optional[int]
+	slot: int = -1
+	fed: int = 0                                          # tokens in the cache
+	out: List[int] = field(default_factory=list)
+	pages: List[int] = field(default_factory=list)
+
+	@property
+	def pending(self) -> int:
+		"""Tokens that are known and not yet in the cache."""
+		return len(self.prompt) + len(self.out) - self.fed
+
+
+class PagedEngine:
+	"""pages: of page_size tokens each, shared by all requests.  requests: how many may run at once.  max_seq: longest request, its generated
+	tokens included (rotary tables, columns of the block table).  portion: prompt tokens per step; longer prompts take several steps, in which the
+	others go on decoding."""
+
+	def __init__(self, model, pages: int, page_size: int = 16, requests: int = 16, max_seq: Optional[int] = None, portion: int = 2048, use_graph: bool = True):
+		if getattr(model, 'tp_world', 1) != 1:
+			raise ValueError('PagedEngine serves models that are not sharded')
+		for layer in model.model.layers:
+			if not isinstance(layer.self_attn, QuantLlamaAttention):
+				raise ValueError('PagedEngine: run make_quant_attn first')
+		if pages < 1 or page_size < 1 or not 1 <= requests <= MAX_REQUESTS or portion < 1:
+			raise ValueError(f'PagedEngine: {pages} pages of {page_size}, {requests} requests, portions of {portion}')
+		self.model, self.cfg = model, model.config
+		self.device = model.lm_head.weight.device
+		self.page_size, self.portion, self.use_graph = page_size, portion, use_graph
+		self.max_seq = max_seq or self.cfg.max_position_embeddings
+		attn = model.model.layers[0].self_attn
+		self.heads, self.dim = attn.num_heads, attn.head_dim
+		shape = (pages, self.heads, page_size, self.dim)
+		zeros = lambda *s, dtype=torch.float16: torch.zeros(s, dtype=dtype, device=self.device)
+		self.kcache = [zeros(*shape) for _ in model.model.layers]
+		self.vcache = [zeros(*shape) for _ in model.model.layers]
+		self.cos, self.sin = attn.tables(self.device, self.max_seq)
+		self.table = zeros(requests, -(-self.max_seq // page_size), dtype=torch.int32)
+		# what a step reads: cached and new tokens per slot, tokens of the rows, free pages in the order in which they are taken
+		self.past, self.new = zeros(requests, dtype=torch.int32), zeros(requests, dtype=torch.int32)
+		self.tok = zeros(requests, dtype=torch.int64)
+		self.pool, self.head = zeros(pages, dtype=torch.int32), zeros(1, dtype=torch.int32)
+		self.free: List[int] = list(range(pages))
+		self.reserved = 0                                    # pages that running requests may still take
+		self.slots: List[Optional[_Request]] = [None] * requests
+		self.waiting: List[_Request] = []
+		self.results: Dict[int, List[int]] = {}
+		self._numbers = 0
+		self._graphs: Dict[int, torch.cuda.CUDAGraph] = {}
+		self._decoding = None                                # the requests that the device buffers are set up for
+
+	# -- requests ------------------------------------------------------------------------------------
+	def _needs(self, tokens: int) -> int:
+		return -(-tokens // self.page_size)
+
+	def add(self, prompt: Sequence[int], steps: int, stop: Optional[int] = None) -> int:
+		"""Queues a request for `steps` tokens behind `prompt` (fewer when `stop` comes up); returns its number."""
+		prompt = [int(t) for t in prompt]
+		total = len(prompt) + steps - 1                      # (the last token is not fed)
+		if not prompt or steps < 1:
+			raise ValueError('a request has a prompt of one token at least and generates one token at least')
+		if min(prompt) < 0 or max(prompt) >= self.cfg.vocab_size:
+			raise ValueError(f'tokens lie in 0 .. {self.cfg.vocab_size - 1}')
+		if total > self.max_seq:
+			raise ValueError(f'{total} positions, the engine was built for max_seq = {self.max_seq}')
+		if self._needs(total) > self.kcache[0].shape[0]:
+			raise ValueError(f'{self._needs(total)} pages, the engine has {self.kcache[0].shape[0]}')
+		self._numbers += 1
+		self.waiting.append(_Request(self._numbers, prompt, int(steps), stop))
+		return self._numbers
+
+	@property
+	def busy(self) -> bool:
+		return bool(self.waiting) or any(r is not None for r in self.slots)
+
+	def _admit(self):
+		"""Requests start in the order in which they came, when a slot and the pages of their whole length are free."""
+		for slot, r in enumerate(self.slots):
+			if r is None and self.waiting:
+				need = self._needs(len(self.waiting[0].prompt) + self.waiting[0].steps - 1)
+				if need > len(self.free) - self.reserved:
+					return
+				r = self.waiting.pop(0)
+				r.slot, self.slots[slot] = slot, r
+				self.reserved += need
+
+	def _finish(self, r: _Request):
+		self.free += r.pages
+		self.reserved -= self._needs(len(r.prompt) + r.steps - 1) - len(r.pages)
+		self.slots[r.slot] = None
+		self.results[r.number] = r.out
+
+	# -- a step --------------------------------------------------------------------------------------
+	@torch.no_grad()
+	def step(self) -> List[Tuple[int, int]]:
+		"""One step: every running request feeds its next token or a portion of its prompt.  Returns (request, token) for those that have
+		generated one."""
+		self._admit()
+		running = [r for r in self.slots if r is not None]
+		if not running:
+			return []
+		left, feed = self.portion, []
+		for r in running:                                    # single tokens always go on; portions share what a step may take
+			n = r.pending
+			if n > 1:
+				n = min(n, left)
+				left -= n
+			feed.append(n)
+		active = [(r, n) for r, n in zip(running, feed) if n]
+		decode = all(r.pending == 1 and n == 1 for r, n in zip(running, feed))
+		logits_rows = self._decode(active) if decode else self._mixed(active)
+		for r, n in active:
+			taken = self._needs(r.fed + n) - len(r.pages)
+			r.pages += self.free[:taken]
+			del self.free[:taken]
+			self.reserved -= taken
+			r.fed += n
+		tokens = logits_rows.tolist()                        # (waits for the device)
+		done = []
+		for (r, n), t in zip(active, tokens):
+			if r.fed < len(r.prompt):
+				continue                                      # a portion inside the prompt
+			r.out.append(int(t))
+			done.append((r.number, int(t)))
+			if len(r.out) == r.steps or t == r.stop:
+				self._finish(r)
+				self._decoding = None
+		return done
+
+	def _upload(self, active, last: int):
+		"""Lengths of the slots 0 .. last - 1 and the pages that the step takes."""
+		past, new = [0] * last, [0] * last
+		for r, n in active:
+			past[r.slot], new[r.slot] = r.fed, n
+		ints = torch.tensor(past + new + self.free, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
+		self.past[:last], self.new[:last] = ints[:last], ints[last:2 * last]
+		self.pool[:len(self.free)] = ints[2 * last:]
+		self.head.zero_()
+
+	def _plan(self, last: int, rows: int, max_new: int):
+		return paged_plan(self.past[:last], self.new[:last], self.table[:last], self.kcache[0], rows, self.heads, pool=self.pool, head=self.head, max_new=max_new)
+
+	def _layers(self, tokens: torch.Tensor, plan) -> torch.Tensor:
+		m, H, D = self.model.model, self.heads, self.dim
+		h = m.embed_tokens(tokens)
+		rows = h.shape[0]
+		for i, layer in enumerate(m.layers):
+			attn = layer.self_attn
+			qkv = attn.qkv_proj(rmsnorm_kernel(h, layer.input_layernorm.weight, layer.input_layernorm.variance_epsilon)).view(rows, 3, H, D)
+			q = paged_append(qkv[:, 0], qkv[:, 1], qkv[:, 2], self.kcache[i], self.vcache[i], plan, self.cos, self.sin)
+			o = paged_attention(q, self.kcache[i], self.vcache[i], plan)
+			h = attn.o_proj(o.view(rows, H * D), residual=h)
+			x = rmsnorm_kernel(h, layer.post_attention_layernorm.weight, layer.post_attention_layernorm.variance_epsilon)
+			h = layer.mlp(x, residual=h) if hasattr(layer.mlp, 'intermediate') else h + layer.mlp(x)
+		return h
+
+	def _greedy(self, h: torch.Tensor) -> torch.Tensor:
+		norm = self.model.model.norm
+		return self.model.lm_head(rmsnorm_kernel(h.contiguous(), norm.weight, norm.variance_epsilon)).argmax(-1)
+
+	def _mixed(self, active) -> torch.Tensor:
+		"""A step with portions of prompts."""
+		last = max(r.slot for r, _ in active) + 1
+		self._upload(active, last)
+		self._decoding = None
+		ids, ends = [], []
+		for r, n in active:                                  # (in the order of their slots, as the rows are)
+			known = r.prompt + r.out
+			ids += known[r.fed:r.fed + n]
+			ends.append(len(ids) - 1)
+		both = torch.tensor(ids + ends, dtype=torch.int64).pin_memory().to(self.device, non_blocking=True)
+		h = self._layers(both[:len(ids)], self._plan(last, len(ids), max(n for _, n in active)))
+		return self._greedy(h.index_select(0, both[len(ids):]))
+
+	def _decode_body(self, last: int):
+		plan = self._plan(last, last, 1)
+		self.past[:last] += self.new[:last]
+		tok = self._greedy(self._layers(self.tok[:last], plan))
+		self.tok[:last].copy_(tok)
+		self.head.copy_(plan.head)                           # (behind the plan's own reading of it)
+
+	def _decode(self, active) -> torch.Tensor:
+		"""A step of single tokens; as long as the same requests run, the device buffers carry on by themselves."""
+		last = max(r.slot for r, _ in active) + 1
+		running = [r.number for r, _ in active]
+		if self._decoding != running:
+			self._upload(active, last)
+			known = [(r.prompt + r.out)[r.fed] for r, _ in active]
+			self.tok[:len(active)] = torch.tensor(known, dtype=torch.int64).pin_memory().to(self.device, non_blocking=True)
+			self._decoding = running
+		if not self.use_graph:
+			self._decode_body(last)
+		else:
+			if last not in self._graphs:
+				self._graphs[last] = self._capture(last)
+			self._graphs[last].replay()
+		return self.tok[:len(active)]
+
+	def _capture(self, last: int):
+		# The trial run writes pages and cache rows that the first real step writes again.
+		state = (self.past, self.tok, self.head)
+		saved = [t.clone() for t in state]
+		s = torch.cuda.Stream(self.device)
+		s.wait_stream(torch.cuda.current_stream(self.device))
+		g = torch.cuda.CUDAGraph()
+		with torch.cuda.stream(s):
+			self._decode_body(last)
+			for t, old in zip(state, saved):
+				t.copy_(old)
+			s.synchronize()
+			with torch.cuda.graph(g, stream=s):
+				self._decode_body(last)
+		torch.cuda.current_stream(self.device).wait_stream(s)
+		return g
+
+	# -- convenience ---------------------------------------------------------------------------------
+	@torch.no_grad()
+	def generate(self, prompts: Sequence[Sequence[int]], steps: int, stop: Optional[int] = None) -> List[List[int]]:
+		"""Greedy generation for prompts of any lengths: the generated tokens of each."""
+		from . import _lib
+		numbers = [self.add(p, steps, stop) for p in prompts]
+		while self.busy:
+			self.step()
+		status = _lib.kernel_status(self.device)
+		if status != 0:
+			raise _lib.GptqB200Error(f'a kernel reported status {status} (see _lib.kernel_status)')
+		return [self.results.pop(n) for n in numbers]
+
+	def close(self):
+		"""Releases the captured graphs."""
+		self._graphs.clear()

@@ -8,7 +8,7 @@ from typing import Callable, Dict, Optional, Tuple
 
 import torch
 
-from . import befalix, lifinex, llama, loader
+from . import befalix, lifinex, llama, loader, paged_engine
 
 
 @dataclass(frozen=True)
@@ -18,6 +18,7 @@ class Architecture:
 	engine: Callable                     # (model, batch, max_seq, use_graph=...) -> StaticEngine
 	dtypes: Tuple[torch.dtype, ...]      # the first one is the default
 	libraries: Tuple[str, ...]           # build targets whose kernels it runs on
+	paged: Optional[Callable] = None     # (model, pages, ...) -> PagedEngine, where requests of different lengths are served
 
 
 ARCHITECTURES: Dict[str, Architecture] = {}
@@ -27,7 +28,8 @@ def register(arch: Architecture):
 	ARCHITECTURES[arch.name] = arch
 
 
-register(Architecture('LlamaForCausalLM', lambda ck, device, dtype: loader.load_quant(str(ck), device=device), llama.DecodeEngine, (torch.float16,), ('gptq',)))
+register(Architecture('LlamaForCausalLM', lambda ck, device, dtype: loader.load_quant(str(ck), device=device), llama.DecodeEngine, (torch.float16,), ('gptq',),
+					  paged_engine.PagedEngine))
 register(Architecture(befalix.ARCHITECTURE, befalix.load_befalix, befalix.BefalixEngine, (torch.bfloat16, torch.float32), ('dense',)))
 register(Architecture(lifinex.ARCHITECTURE, lifinex.load_lifinex, lifinex.LifinexEngine, (torch.bfloat16, torch.float32), ('dense',)))
 
@@ -57,3 +59,11 @@ def load_model(checkpoint, device='cuda', dtype: Optional[torch.dtype] = None):
 def make_engine(model, batch: int, max_seq: int, **kw):
 	"""The engine that serves `model` (see StaticEngine)."""
 	return ARCHITECTURES[getattr(type(model), 'architecture', 'LlamaForCausalLM')].engine(model, batch=batch, max_seq=max_seq, **kw)
+
+
+def make_paged_engine(model, pages: int, **kw):
+	"""The engine that serves requests of different lengths from a cache in pages (see PagedEngine)."""
+	arch = ARCHITECTURES[getattr(type(model), 'architecture', 'LlamaForCausalLM')]
+	if arch.paged is None:
+		raise ValueError(f'{arch.name} is not served from a cache in pages: give it prompts of equal length')
+	return arch.paged(model, pages, **kw)

@@ -1,5 +1,5 @@
 /*
- * paged_b200.h — C ABI of libpaged_b200.so: serving from a key / value cache in pages on NVIDIA B200 (sm_100a).
+ * paged_b200.h — C ABI of libgptq_b200.so, continued: serving from a key / value cache in pages on NVIDIA B200 (sm_100a).
  * Block tables and slot maps from request lengths, rotation of queries and keys with the store of the new rows, attention of the
  * new tokens of every request over its pages.
  *

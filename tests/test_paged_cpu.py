@@ -12,7 +12,7 @@ ROOT = Path(__file__).resolve().parent.parent
 @pytest.fixture(scope='module')
 def lib():
 	from gptq_triton_b200 import _paged, build
-	build.build(only=['paged'])
+	build.build(only=['gptq'])
 	return _paged.lib()
 
 
