@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const paged_plan_t p, 
 			if (blockIdx.x == 0) {
 				p.row_start[r] = s_start[r];
 				p.lens[r] = len;
-				if (len < l.past + l.fresh) bad |= PAGED_NO_ROOM;
+				if (len < l.past + l.fresh || l.fresh > p.max_fresh) bad |= PAGED_NO_ROOM;
 			}
 		}
 		if (tid == 0 && blockIdx.x == 0) {

@@ -78,7 +78,8 @@ def paged_plan(past: torch.Tensor, new: torch.Tensor, table: torch.Tensor, cache
 	that the new tokens need are written into it in place, requests in order; plan.head is the place behind them (a tensor of its own,
 	so the same call again gives the same plan).  Without, the table must name all pages.
 	cache: a key cache tensor of the layers, for its sizes and type.  rows: rows of q, k and v, at least the sum of `new`; rows left over
-	get slot -1.  heads: query heads.  max_new: no request has more new tokens (default: rows); only speed depends on it.
+	get slot -1.  heads: query heads.  max_new: no request has more new tokens (default: rows), which spares launches and time; one
+	that has sets status 8.
 	"""
 	if cache.is_cuda:
 		code = _paged.DTYPE_CODE.get(cache.dtype)

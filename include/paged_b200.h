@@ -24,7 +24,7 @@ extern "C" {
 #define PAGED_MAX_DIM 256
 /* bits of the status word (a run that meets one goes on without touching memory that is not its own) */
 #define PAGED_BAD_INDEX 4              /* a page, position or slot outside the cache or the tables, or a negative length */
-#define PAGED_NO_ROOM 8                /* pages of the pool, columns of the table or rows ran out */
+#define PAGED_NO_ROOM 8                /* pages of the pool, columns of the table or rows ran out, or a request has more than max_fresh new tokens */
 
 /* The plan of one step.  Request r has past[r] tokens in the cache and gets fresh[r] new ones (0 is allowed).  Rows are the new
  * tokens, request after request; rows behind the last one get slot -1 and position 0.
@@ -44,7 +44,7 @@ typedef struct {
 	int32_t *positions;                /* [rows] */
 	int64_t *slots;                    /* [rows] */
 	int heads, kv_heads, dim;
-	int max_fresh;                     /* no request has more new tokens (rows, if nothing is known) */
+	int max_fresh;                     /* no request has more new tokens (rows, if nothing is known); one that has sets PAGED_NO_ROOM */
 	int32_t *work;
 	int *status;
 } paged_plan_t;

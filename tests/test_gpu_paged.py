@@ -78,7 +78,7 @@ def test_plan_of_nothing():
 	assert plan.row_start.tolist() == [0] and plan.slots.numel() == 0
 
 
-@pytest.mark.parametrize('what,bits', [('pool', 8), ('table', 8), ('rows', 8), ('negative', 4), ('page', 4), ('head', 4), ('huge', 4)])
+@pytest.mark.parametrize('what,bits', [('pool', 8), ('table', 8), ('rows', 8), ('negative', 4), ('page', 4), ('head', 4), ('huge', 4), ('more', 8)])
 def test_plan_without_room(what, bits):
 	"""What only the device sees sets the status; slots of such tokens are -1 and nothing else is written."""
 	from gptq_triton_b200 import paged_plan
@@ -101,7 +101,7 @@ def test_plan_without_room(what, bits):
 	elif what == 'huge':
 		past = [2000000000, 3]
 	cache = torch.empty((8, 1, page, 8), dtype=torch.float16, device=DEV)
-	plan = paged_plan(i32(past), i32(new), i32(table), cache, rows, 1, pool=i32(pool), head=i32(head))
+	plan = paged_plan(i32(past), i32(new), i32(table), cache, rows, 1, pool=i32(pool), head=i32(head), max_new=20 if what == 'more' else None)
 	torch.cuda.synchronize()
 	assert status() & bits
 	s = plan.slots.tolist()
