@@ -126,6 +126,7 @@ __device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, co
 		}
 		units = add_to(units, total, PL_LIMIT);
 	}
+	if (units >= PL_LIMIT && tid == 0) atomicOr(p.status, PAGED_NO_ROOM);          // (more keys than the lists count: 10^9 blocks)
 	__syncthreads();
 	if (E > PL_NEAR && part > 0) return;                   // (the other entries are in global memory, where part 0 has written them)
 	if (E > PL_NEAR) parts = 1;

@@ -40,6 +40,7 @@ class PagedPlan:
 	rows: int
 	max_new: int
 	serves: tuple
+	native: tuple = ()            # the same for native code: type code, heads, kv_heads, page, pages, dim, rows, address of the status word
 
 
 def _int32(t: torch.Tensor, name: str, dims: int, device):
@@ -82,12 +83,12 @@ def paged_plan(past: torch.Tensor, new: torch.Tensor, table: torch.Tensor, cache
 	that has sets status 8.
 	"""
 	if cache.is_cuda:
-		code = _paged.DTYPE_CODE.get(cache.dtype)
-		served = _paged.native().paged_plan(past, new, table, cache, code, rows, heads, pool, head, rows if max_new is None else min(max_new, rows), _paged.status_ptr(cache.get_device()))
+		dt = cache.dtype
+		code, most, status = _paged.DTYPE_CODE.get(dt), rows if max_new is None else min(max_new, rows), _paged.status_ptr(cache.get_device())
+		served = _paged.native().paged_plan(past, new, table, cache, code, rows, heads, pool, head, most, status)
 		if served is not None:
-			row_start, lens, positions, slots, nxt, work = served
 			pages, kv_heads, page, dim = cache.shape
-			return PagedPlan(table, row_start, lens, positions, slots, nxt, work, rows, rows if max_new is None else min(max_new, rows), (heads, kv_heads, page, pages, dim, cache.dtype))
+			return PagedPlan(table, *served, rows, most, (heads, kv_heads, page, pages, dim, dt), (code, heads, kv_heads, page, pages, dim, rows, status))
 	require_cuda(past, new, table, cache, pool, head)
 	dev = cache.device
 	_cache(cache, 'cache')
@@ -100,6 +101,8 @@ def paged_plan(past: torch.Tensor, new: torch.Tensor, table: torch.Tensor, cache
 		raise ValueError(f'past, new and table must speak of the same requests, at most {_paged.MAX_REQUESTS}: {R}, {new.numel()}, {table.shape[0]}')
 	if rows < 0 or rows >= 1 << 30 or kv_heads < 1 or heads < 1 or heads % kv_heads or page < 1 or dim < 1 or table.shape[1] < 1:
 		raise ValueError(f'paged_plan: {rows} rows, {heads} heads over {kv_heads} key heads, pages of {page} rows of {dim}, {table.shape[1]} table columns')
+	if R > 1 and table.stride(0) < table.shape[1]:
+		raise ValueError(f'table: rows that overlap (strides {table.stride()})')
 	if (pool is None) != (head is None):
 		raise ValueError('pool and head go together')
 	if pool is not None:
@@ -128,7 +131,8 @@ def paged_plan(past: torch.Tensor, new: torch.Tensor, table: torch.Tensor, cache
 	a.heads, a.kv_heads, a.dim, a.max_fresh, a.work, a.status = heads, kv_heads, dim, max_new, ptr(work), _paged.status_ptr(dev.index)
 	with _On(dev):
 		_paged.check(lib.paged_plan(ctypes.byref(a), _paged.DTYPE_CODE[cache.dtype], stream_ptr(dev)), 'paged_plan')
-	return PagedPlan(table, row_start, lens, positions, slots, None if pool is None else nxt, work, rows, max_new, (heads, kv_heads, page, pages, dim, cache.dtype))
+	return PagedPlan(table, row_start, lens, positions, slots, None if pool is None else nxt, work, rows, max_new, (heads, kv_heads, page, pages, dim, cache.dtype),
+					 (_paged.DTYPE_CODE[cache.dtype], heads, kv_heads, page, pages, dim, rows, _paged.status_ptr(dev.index)))
 
 
 def _caches(k_cache, v_cache, plan: PagedPlan, what: str):
@@ -161,14 +165,13 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: tor
 	q: [rows, heads, dim], k, v: [rows, kv_heads, dim], any strides with neighbouring entries (columns of a fused projection).  cos, sin:
 	[positions, rot] in the type of q, rotate-half convention as rope_tables() gives them; rot < dim turns the first entries of a head
 	only; without tables nothing is turned.  Rows with slot -1 are not stored; a position outside the tables sets status 4, its row is
-	turned as position 0 and not stored.  `out` may be q itself (contiguous).
+	turned as position 0 and not stored.  Slots are distinct unless the block table gives one page to two requests that write to it: which row
+	such a place then holds is open.  `out` may be q itself (contiguous).
 	"""
+	served = _paged.native().paged_append(q, k, v, k_cache, v_cache, cos, sin, out, plan.positions, plan.slots, *plan.native)
+	if served is not None:
+		return served
 	heads, kv_heads, page, pages, dim, dt = plan.serves
-	if q.is_cuda:
-		served = _paged.native().paged_append(q, k, v, k_cache, v_cache, cos, sin, out, plan.positions, plan.slots, _paged.DTYPE_CODE[dt], heads, kv_heads, page, pages, dim, plan.rows,
-											  _paged.status_ptr(q.get_device()))
-		if served is not None:
-			return served
 	require_cuda(q, k, v, k_cache, v_cache, cos, sin, out)
 	_caches(k_cache, v_cache, plan, 'paged_append')
 	_rows(q, 'q', plan, heads)
@@ -200,16 +203,15 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 	"""softmax(scale q k^T) v of every new token over the positions up to its own, [rows, heads, dim].
 
 	q: [rows, heads, dim] (rotated); query head h reads key head h // (heads // kv_heads).  scale: positive, default 1 / sqrt(dim).
-	Rows behind the last one in use are left as they are (`out`) or have no particular value.  Values of positions behind a request's last
-	one do not count, whatever the pages hold there.
+	Rows behind the last one in use are left as they are (`out`, which may be q itself) or have no particular value.  Values of positions
+	behind a request's last one do not count, whatever the pages hold there.  A value of a new token that is not finite can make earlier
+	rows of the same step and request NaN (a weight of zero times it), as it does in the formula's products.
 	"""
 	heads, kv_heads, page, pages, dim, dt = plan.serves
 	scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-	if q.is_cuda:
-		served = _paged.native().paged_attention(q, k_cache, v_cache, out, scale, plan.table, plan.row_start, plan.lens, plan.work, plan.max_new, _paged.DTYPE_CODE[dt], heads, kv_heads, page,
-												 pages, dim, plan.rows, _paged.status_ptr(q.get_device()))
-		if served is not None:
-			return served
+	served = _paged.native().paged_attention(q, k_cache, v_cache, out, scale, plan.table, plan.row_start, plan.lens, plan.work, plan.max_new, *plan.native)
+	if served is not None:
+		return served
 	require_cuda(q, k_cache, v_cache, out)
 	_caches(k_cache, v_cache, plan, 'paged_attention')
 	_rows(q, 'q', plan, heads)

@@ -34,7 +34,7 @@ def test_refusals_of_the_plan(step):
 						  (dict(heads=7), ValueError), (dict(heads=0), ValueError), (dict(rows=-1), ValueError), (dict(cache=k[0]), ValueError), (dict(cache=k.double()), ValueError),
 						  (dict(cache=k.transpose(2, 3)), ValueError), (dict(cache=k[..., ::2]), ValueError), (dict(pool=pool), ValueError), (dict(head=head), ValueError), (dict(pool=pool, head=i32([0, 1])), ValueError),
 						  (dict(pool=pool.long(), head=head), ValueError), (dict(max_new=-1), ValueError), (dict(past=torch.zeros(3, dtype=torch.int32)), _lib.GptqB200Error),
-						  (dict(past=i32([0] * 8193), new=i32([0] * 8193), table=i32([[0]] * 8193)), ValueError), (dict(past=i32(step.past * 2)[::2]), ValueError)):
+						  (dict(past=i32([0] * 8193), new=i32([0] * 8193), table=i32([[0]] * 8193)), ValueError), (dict(past=i32(step.past * 2)[::2]), ValueError), (dict(table=i32(step.table)[:1].expand(3, -1)), ValueError)):
 		with pytest.raises(error):
 			G.paged_plan(**{**ok, **change})
 
@@ -195,6 +195,51 @@ def test_captured_steps_follow_the_lengths():
 			error = (g.out.cpu().double() - want).abs()
 			assert (error <= bound(want, absolute, score, dim, max(lens), torch.float16)).all(), i
 	status()
+
+
+@pytest.mark.parametrize('new', [1, 100])
+def test_cache_of_more_than_two_thousand_million_entries(new):
+	"""Pages whose first entry lies beyond 2^31: rows that are stored and read there."""
+	heads, dim, page = 4, 128, 16
+	pages = (2 ** 31 + 2 ** 28) // (heads * page * dim)
+	s = Step([40], [new], heads, heads, dim, page, 'fp16', filled=False, fill=0.0)
+	k, v = (torch.empty((pages, heads, page, dim), dtype=torch.float16, device=DEV) for _ in range(2))
+	used = -(-(40 + new) // page)
+	own = [pages - 1 - 3 * i for i in range(used)]
+	for i, mine in enumerate(own):
+		k[mine], v[mine] = s.k[s.table[0][i]].to(DEV), s.v[s.table[0][i]].to(DEV)
+	s.table = [own]
+	q, kn, vn = s.parts(s.qkv.to(DEV))
+	plan = G.paged_plan(s.ints([40]), s.ints([new]), s.ints([own]), k, s.rows, heads)
+	assert plan.slots.tolist() == [own[p // page] * page + p % page for p in range(40, 40 + new)]
+	G.paged_append(q, kn, vn, k, v, plan)
+	out = G.paged_attention(q, k, v, plan)
+	small_k, small_v = (torch.stack([t[m] for m in own]).cpu() for t in (k, v))
+	j = torch.arange(40, 40 + new)
+	assert torch.equal(small_k[j // page, :, j % page], s.parts()[1]) and torch.equal(small_v[j // page, :, j % page], s.parts()[2])
+	want, absolute, score = O.attention(s.parts()[0], small_k, small_v, [list(range(used))], [0, new], [40 + new])
+	assert ((out.cpu().double() - want).abs() <= bound(want, absolute, score, dim, 40 + new, torch.float16)).all()
+
+
+@pytest.mark.parametrize('new', [[1, 1], [40, 70]])
+def test_results_in_the_place_of_the_queries(new):
+	s = Step([300, 20], new, 8, 2, 64, 16, 'bf16')
+	k, v = s.k.to(DEV), s.v.to(DEV)
+	q = s.parts(s.qkv.to(DEV))[0].contiguous()
+	plan = make_plan(s, k)
+	want = G.paged_attention(q, k, v, plan)
+	assert G.paged_attention(q, k, v, plan, out=q) is q and torch.equal(q, want)
+
+
+def test_a_page_in_two_tables():
+	"""Requests that share the pages of a common beginning."""
+	s = Step([64, 64], [1, 20], 8, 2, 64, 16, 'fp16')
+	for c in range(4):
+		s.table[1][c] = s.table[0][c]
+	k, v = s.k.to(DEV), s.v.to(DEV)
+	out = G.paged_attention(s.parts(s.qkv.to(DEV))[0], k, v, make_plan(s, k))
+	want, absolute, score = O.attention(s.parts()[0], s.k, s.v, s.table, [0, 1, 21], [65, 84])
+	assert ((out.cpu().double() - want).abs() <= bound(want, absolute, score, 64, 84, torch.float16)).all()
 
 
 def test_another_stream(step):
