@@ -45,9 +45,9 @@ inline __host__ __device__ int pg_few(int group) { return group > 1 ? 32 : PG_RO
 constexpr int PG_TILE = 256, PG_TILE_KEYS = 128, PG_TILE_SLOTS = 148;
 inline __host__ __device__ int pg_begin(int kind) { return kind ? 2 : 1; }
 
-struct PgList {                        // of one of the two kernels; behind it in `work`: starts, entries, order
+struct PgList {                        // of one of the two kernels; behind it in `work`: starts, entries, sorted
 	int entries;
-	int whole;                          // slots take whole jobs by `order` instead (tile kernel)
+	int whole;                          // slots take whole jobs in the order of `sorted` instead (tile kernel)
 	int64_t per, total;                 // length of a slot's share, of all jobs
 	int cuts[2];                        // slots in which a job begins that ends in a later one: how many, in the two parts of the list
 };
@@ -82,7 +82,7 @@ struct PgWork {
 	PgList *list;                       // [2]
 	PgStart *starts[2];                 // [slots + 1]
 	PgEntry *entries[2];
-	int *order;
+	PgEntry *sorted;                    // of the tile kernel, the longest first
 	int *cuts[2];                       // [2 PG_SLOTS], [2 PG_TILE_SLOTS]: the slots of both parts
 	int cap[2];
 	int64_t ints;
@@ -102,8 +102,8 @@ inline __host__ __device__ PgWork pg_work(int32_t *base, int requests, int rows,
 	at += 8 * (int64_t)w.cap[0];
 	w.entries[1] = reinterpret_cast<PgEntry *>(base + at);
 	at += 8 * (int64_t)w.cap[1];
-	w.order = base + at;
-	at += w.cap[1];
+	w.sorted = reinterpret_cast<PgEntry *>(base + at);
+	at += 8 * (int64_t)w.cap[1];
 	w.cuts[0] = base + at;
 	at += 2 * PG_SLOTS;
 	w.cuts[1] = base + at;

@@ -89,6 +89,13 @@ constexpr int PL_KEEP = 4096;          // entries whose places and lengths are k
 constexpr int PL_NEAR = 1024;          // ... and those that are kept there whole
 constexpr int PL_PARTS = 2;            // CTAs that share the starts of the kernel for few rows
 
+// (16 bytes at a time: word by word the stores of the lists take half of the kernel's time)
+__device__ __forceinline__ void put(PgEntry *to, const PgEntry &x) {
+	int4 *dst = reinterpret_cast<int4 *>(to);
+	dst[0] = make_int4(x.request, x.tile, x.blocks, x.first);
+	dst[1] = make_int4(x.row, x.fresh, x.len, x.seen);
+}
+
 // The work list of one kernel.  s_tiles [R + 1]: tiles of the requests before; s_len [R]; s_entry [PL_NEAR], s_first, s_sorted [PL_KEEP].
 // The CTAs that share a list all form it, `part` 0 writes the entries, each its part of the starts.
 __device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, const int *s_start, const int *s_len, const int *s_tiles, PgEntry *s_entry, int *s_first, int *s_sorted, int *s_scan,
@@ -116,11 +123,7 @@ __device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, co
 		scan2(n, none, PL_LIMIT, PL_LIMIT, total, unused, s_scan);
 		if (e < E) {
 			x.first = add_to(units, n, PL_LIMIT);
-			if (part == 0) {
-				int4 *dst = reinterpret_cast<int4 *>(w.entries[kind] + e);
-				dst[0] = make_int4(x.request, x.tile, x.blocks, x.first);
-				dst[1] = make_int4(x.row, x.fresh, x.len, x.seen);
-			}
+			if (part == 0) put(w.entries[kind] + e, x);
 			if (e < PL_NEAR) s_entry[e] = x;
 			if (e < PL_KEEP) s_first[e] = x.first;
 		}
@@ -156,12 +159,13 @@ __device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, co
 			__syncthreads();
 			// (tiles of one length are in no particular order: which slot takes one changes no result)
 			for (int e = tid; e < E; e += PL_THREADS) {
-				const int n = blocks_of(e), at = atomicAdd(&s_hist[bucket(n)], 1);
-				w.order[at] = e;
-				s_sorted[at] = n + pg_begin(1);
+				const PgEntry x = e < PL_NEAR ? s_entry[e] : w.entries[1][e];
+				const int at = atomicAdd(&s_hist[bucket(x.blocks)], 1);
+				put(w.sorted + at, x);
+				s_sorted[at] = x.blocks + pg_begin(1);
 			}
 		} else {
-			for (int e = tid; e < E; e += PL_THREADS) w.order[e] = e;
+			for (int e = tid; e < E; e += PL_THREADS) put(w.sorted + e, w.entries[1][e]);
 		}
 		__syncthreads();
 		const int64_t items = (int64_t)E * p.kv_heads;
@@ -212,10 +216,8 @@ __device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, co
 			s.block = max((int)(rest - (int64_t)s.kv * n) - pg_begin(kind), 0);
 		}
 		if (c <= slots) {
-			int4 *dst = reinterpret_cast<int4 *>(w.starts[kind] + c);          // (16 bytes at a time: word by word these stores take half of the kernel's time)
-			dst[0] = make_int4(s.entry, s.kv, s.block, 0);
-			dst[1] = make_int4(s.job.request, s.job.tile, s.job.blocks, s.job.first);
-			dst[2] = make_int4(s.job.row, s.job.fresh, s.job.len, s.job.seen);
+			*reinterpret_cast<int4 *>(w.starts[kind] + c) = make_int4(s.entry, s.kv, s.block, 0);
+			put(&w.starts[kind][c].job, s.job);
 		}
 		// the first cut of a job lies less than a share behind its begin
 		int at = s.entry >= 0 && s.block > 0 && s.block <= per, none = 0, count, unused;

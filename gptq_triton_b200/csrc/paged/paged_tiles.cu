@@ -5,13 +5,19 @@
 // softmax, O += P V; while the softmax warps of one side work, the tensor cores work for the other.
 //   softmax warps   four per side, a thread owns a row: 128 scores from tensor memory, mask where the block crosses what the row sees,
 //                   weights in the type of the values back to the columns of the scores (they are the A operand of P V there)
-//   TMA warp        key and value blocks through one ring; a lane per page and 64 columns of a block, so pages of 8 rows and more serve;
-//                   pages behind what the tile sees, or that do not exist, are asked for outside the tensor and arrive as zeros
-//   MMA warp        both sides in turn: P V of this block, Q K^T of the next
+//   TMA warp        key and value blocks through one ring; a lane knows the page of its part of a block, so pages of 8 rows and more serve, one
+//                   lane issues; pages behind what the tile sees, or that do not exist, are asked for outside the tensor and arrive as zeros
+//   MMA lane        both sides in turn: P V of this block in two halves, as the weights come, Q K^T of the next
 // O is rescaled only when a row's maximum has grown by more than 2^8.  fp32 sums; weights are rounded to the type of the values, their
 // sum is taken before that.  Values behind the last key seen are zeroed in shared memory: a weight of zero times NaN would be NaN.
-// CTAs stay for the whole launch and take tiles, or equal ranges of all key blocks (paged_plan); ranges that end inside a tile leave
-// partial results, which tile_join_kernel adds up.  Every wait is bounded.
+// CTAs stay for the whole launch and take whole jobs, or equal shares of all (paged_plan); cut jobs leave partial results, which
+// join_kernel adds up.  Every wait is bounded.
+//
+// 512 tokens behind 30 000, 64 heads over 8 of 128, bf16: 452 us inside a graph, 1 124 TFLOP/s; 2 047 tokens of 32 heads 49 us; twelve prompts of 90 to
+// 3 000 tokens 157 us.  Bound by the chain of a block (scores, maximum, weights, products; 3 450 cycles for two sides that take turns, of
+// which the tensor cores are busy for 58 %) and the clock under this load: without the exponentials it takes 440 us, with next to no MMAs
+// 377, with neither 298.  Measured against this form, us: MMAs behind `lane == 0` 565, two threads per row 473, an MMA warp per side 505 (both
+// sides then fall into step), scores of 64 keys in two buffers 510, a quarter of the exponentials on the FMA units 468.
 #include <mutex>
 
 #include "../tcgen05.cuh"
@@ -24,7 +30,8 @@ namespace {
 constexpr int TL_SIDE = 128, TL_KEYS = PG_TILE_KEYS;
 constexpr int TL_CHUNK = 128 * 128;                      // bytes of 128 rows of 64 columns
 constexpr int TL_THREADS = 384, TL_TMA = 8, TL_MMA = 9;          // (warps 10 and 11 complete the third warpgroup)
-constexpr int TL_REGS_SOFTMAX = 208, TL_REGS_OTHER = 88;          // of 168 at launch: 2 * 208 + 88 = 3 * 168
+// registers of a thread behind setmaxnreg; what the kernel is launched with has to cover them (tiles_launch looks)
+constexpr int TL_REGS_SOFTMAX = 208, TL_REGS_OTHER = 88, TL_REGS_LAUNCH = (2 * TL_REGS_SOFTMAX + TL_REGS_OTHER) / 3;
 constexpr uint32_t TL_SPIN = 1u << 24;                  // polls of a bounded wait
 
 template <int DP> struct TileShape {
@@ -81,34 +88,30 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
 struct Items {
 	PgEntry e;
 	int kv, j0, j1;                    // key head, blocks of keys
-	const PgEntry *entries;
-	const int *order;
+	const PgEntry *entries, *sorted;
 	PgStart end;                       // where the next slot begins
 	int slot, kv_heads, whole, entry, entry_count, turn;
-	__device__ Items(const PgWork &w, int kvh, int s) : entries(w.entries[1]), order(w.order), slot(s), kv_heads(kvh) {
+	__device__ Items(const PgWork &w, int kvh, int s) : entries(w.entries[1]), sorted(w.sorted), slot(s), kv_heads(kvh) {
+		// (asked for together: which of them count depends on the list)
 		const PgList l = read_list(w.list + 1);
+		const PgStart st = read_start(w.starts[1] + s);
+		const PgEntry first = read_entry(w.sorted + min(s / kvh, w.cap[1] - 1));
+		end = read_start(w.starts[1] + s + 1);
 		whole = l.whole;
 		entry_count = l.entries;
 		turn = 0;
-		kv = j1 = 0;
-		entry = -1;
-		if (!whole) {
-			const PgStart st = read_start(w.starts[1] + s);
-			end = read_start(w.starts[1] + s + 1);
-			entry = st.entry;
-			kv = st.kv;
-			j1 = st.block;
-			e = st.job;
-		}
+		kv = whole ? 0 : st.kv;
+		j1 = whole ? 0 : st.block;
+		entry = whole ? 0 : st.entry;
+		e = whole ? first : st.job;
 	}
 	__device__ bool next() {
 		if (whole) {                     // sorted by length, dealt out forwards and backwards in turn
 			constexpr int slots = PG_TILE_SLOTS;
-			const int i = turn & 1 ? (turn + 1) * slots - 1 - slot : turn * slots + slot;
-			++turn;
-			if (i / kv_heads >= entry_count) return false;
-			kv = i % kv_heads;
-			e = read_entry(entries + __ldcg(order + i / kv_heads));
+			const int i = turn & 1 ? (turn + 1) * slots - 1 - slot : turn * slots + slot, at = i / kv_heads;
+			if (at >= entry_count) return false;
+			kv = i - at * kv_heads;
+			if (turn++) e = read_entry(sorted + at);
 			j0 = 0;
 			j1 = e.blocks;
 			return true;
@@ -525,6 +528,11 @@ int tiles_launch(const paged_attention_t &p, const PgWork &work, bool half, cuda
 	if (int rc = cache_map(p.v_cache, p, p.v_page, p.v_kv, half, &tmv)) return rc;
 	constexpr int smem = TileShape<DP>::SMEM;
 	static_assert(smem + 1024 <= 227 * 1024, "shared memory of a CTA");
+	static const int registers = [] {
+		cudaFuncAttributes attr;
+		return cudaFuncGetAttributes(&attr, tiles_kernel<T, DP>) == cudaSuccess ? attr.numRegs : 0;
+	}();
+	if (registers < TL_REGS_LAUNCH) return GPTQ_ERR_UNSUPPORTED;          // (the softmax warps would wait for registers that nobody gives back)
 	return pg_launch(tiles_kernel<T, DP>, dim3(PG_TILE_SLOTS), TL_THREADS, smem, stream, tmk, tmv, p, work);
 }
 
