@@ -84,7 +84,7 @@ __device__ __forceinline__ Lengths lengths_of(const paged_plan_t &p, int r, int 
 // What the attention sees of a request is at most what its table can name.
 __device__ __forceinline__ int length_seen(const paged_plan_t &p, const Lengths &l) { return (int)min((int64_t)l.past + l.fresh, min((int64_t)p.table_width * p.page, (int64_t)PL_LIMIT)); }
 
-constexpr int PL_JOIN = 6, PL_LEAST = 2;
+constexpr int PL_JOIN = 6;
 constexpr int PL_KEEP = 4096;          // entries whose places and lengths are kept in shared memory
 constexpr int PL_NEAR = 1024;          // ... and those that are kept there whole
 constexpr int PL_PARTS = 2;            // CTAs that share the starts of the kernel for few rows
@@ -134,9 +134,9 @@ __device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, co
 	if (E > PL_NEAR && part > 0) return;                   // (the other entries are in global memory, where part 0 has written them)
 	if (E > PL_NEAR) parts = 1;
 	auto blocks_of = [&](int e) { return e < PL_NEAR ? s_entry[e].blocks : w.entries[kind][e].blocks; };
-	// (a share is longer than what a job costs besides its blocks, so that no two slots begin at the same place; shorter
-	// shares would be mostly partial results)
-	const int64_t total = (int64_t)units * p.kv_heads, per = max((total + slots - 1) / slots, (int64_t)(PL_LEAST + pg_begin(kind)));
+	// A share is longer than what a job costs besides its blocks, so that no two slots begin at the same place.  One block of 16 keys beyond
+	// that for few rows (one token of 32 heads behind 100, us: 1 block 7.2, 2 8.0, 4 10.0; behind 2 100 11.7, 11.7, 11.8).
+	const int64_t total = (int64_t)units * p.kv_heads, per = max((total + slots - 1) / slots, (int64_t)((kind ? 2 : 1) + pg_begin(kind)));
 	int whole = 0;
 	if (kind) {
 		// Whole tiles, the longest first, dealt out to the slots forwards and backwards in turn, unless the longest slot would then work
