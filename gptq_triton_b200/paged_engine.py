@@ -245,7 +245,13 @@ class PagedEngine:
 	def generate(self, prompts: Sequence[Sequence[int]], steps: int, stop: Optional[int] = None) -> List[List[int]]:
 		"""Greedy generation for prompts of any lengths: the generated tokens of each."""
 		from . import _lib
-		numbers = [self.add(p, steps, stop) for p in prompts]
+		numbers = []
+		try:
+			for p in prompts:
+				numbers.append(self.add(p, steps, stop))
+		except Exception:                                     # one is refused: none of them stays queued
+			self.waiting = [r for r in self.waiting if r.number not in numbers]
+			raise
 		while self.busy:
 			self.step()
 		status = _lib.kernel_status(self.device)

@@ -122,3 +122,12 @@ def test_command_line(case, tmp_path, capsys):
 	assert [len(r) for r in rows] == [5, 5, 5]
 	engine = G.PagedEngine(G.load_model(str(tmp_path)), pages=8, max_seq=20)
 	assert engine.generate([[1, 2, 3], [7], [9, 10]], 5) == rows
+
+
+def test_a_refused_prompt_leaves_nothing_queued(case):
+	import gptq_triton_b200 as G
+	cfg, model, prompts, want = case
+	engine = G.PagedEngine(model, pages=64, max_seq=80)
+	with pytest.raises(ValueError):
+		engine.generate([prompts[0], [-1]], STEPS)
+	assert not engine.busy and engine.generate([prompts[1]], STEPS) == [want[1]]
