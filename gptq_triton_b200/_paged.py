@@ -14,6 +14,7 @@ from ._lib import LIB_PATH, GptqB200Error, ptr, register_status_buffer, require_
 CONTROL_BYTES = 16384
 MAX_REQUESTS = 8192
 MAX_DIM = 256
+MAX_PAGE = 1 << 24
 DTYPE_CODE = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 
 _P, _I = c_void_p, c_int

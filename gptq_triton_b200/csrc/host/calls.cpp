@@ -439,7 +439,7 @@ PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
 			table->size(1) < 1 || table->stride(1) != 1 || (table->size(0) > 1 && table->stride(0) < table->size(1)) || !pool != !head || (pool && (pool->dim() != 1 || head->dim() != 1 || head->numel() != 1)) || rows == 0 || most > rows)
 			return nullptr;
 		const int64_t R = past->numel(), pages = cache.t->size(0), kv = cache.t->size(1), page = cache.t->size(2), dim = cache.t->size(3);
-		if (R > PAGED_MAX_REQUESTS || heads < 1 || heads % kv || pages > INT_MAX || page > INT_MAX || table->size(1) > INT_MAX || (pool && pool->numel() > INT_MAX)) return nullptr;
+		if (R > PAGED_MAX_REQUESTS || rows >= 1 << 30 || heads < 1 || heads > 65535 || heads % kv || pages > INT_MAX || page > INT_MAX || table->size(1) > INT_MAX || (pool && pool->numel() > INT_MAX)) return nullptr;
 		const int64_t ints = work_ints((int)R, (int)rows, (int)heads, (int)kv);
 		if (ints < 0) return nullptr;
 		const int64_t at_work = (2 * rows + 3) / 4 * 4, at_start = at_work + ints, at_lens = at_start + R + 1, at_pos = at_lens + R, at_head = at_pos + rows;

@@ -29,6 +29,7 @@ namespace {
 
 bool known(int dtype) { return dtype == PG_BF16 || dtype == PG_F32 || dtype == PG_F16; }
 int size_of(int dtype) { return dtype == PG_F32 ? 4 : 2; }
+bool page_ok(int page) { return page >= 1 && page <= PAGED_MAX_PAGE; }
 bool heads_ok(int heads, int kv_heads) { return kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && heads <= 65535; }
 // heads and pages start on 16 bytes
 bool steps_ok(int64_t a, int64_t b, int dtype) { return a * size_of(dtype) % 16 == 0 && b * size_of(dtype) % 16 == 0; }
@@ -48,7 +49,7 @@ int64_t paged_work_ints(int requests, int rows, int heads, int kv_heads) {
 }
 
 int paged_plan(const paged_plan_t *p, int dtype, void *stream) {
-	if (!p || !known(dtype) || p->requests < 0 || p->requests > PAGED_MAX_REQUESTS || p->rows < 0 || p->page < 1 || p->pages < 0 || p->table_width < 1 || p->table_ld < p->table_width ||
+	if (!p || !known(dtype) || p->requests < 0 || p->requests > PAGED_MAX_REQUESTS || p->rows < 0 || !page_ok(p->page) || p->pages < 0 || p->table_width < 1 || p->table_ld < p->table_width ||
 		!heads_ok(p->heads, p->kv_heads) || !p->row_start || !p->work || !p->status || p->max_fresh < 0 || paged_work_ints(p->requests, p->rows, p->heads, p->kv_heads) < 0)
 		return GPTQ_ERR_INVALID;
 	if (p->requests && (!p->past || !p->fresh || !p->table || !p->lens)) return GPTQ_ERR_INVALID;
@@ -59,7 +60,7 @@ int paged_plan(const paged_plan_t *p, int dtype, void *stream) {
 }
 
 int paged_append(const paged_append_t *p, int dtype, void *stream) {
-	if (!p || !known(dtype) || p->rows < 0 || !heads_ok(p->heads, p->kv_heads) || p->dim < 1 || p->rot < 0 || p->rot > p->dim || p->rot % 2 || p->page < 1 || p->pages < 0 || !p->status)
+	if (!p || !known(dtype) || p->rows < 0 || !heads_ok(p->heads, p->kv_heads) || p->dim < 1 || p->rot < 0 || p->rot > p->dim || p->rot % 2 || !page_ok(p->page) || p->pages < 0 || !p->status)
 		return GPTQ_ERR_INVALID;
 	if (p->rows == 0) return GPTQ_OK;
 	if (!p->q || !p->k || !p->v || !p->q_out || !p->k_cache || !p->v_cache || !p->slots || (p->rot && (!p->cos_t || !p->sin_t || !p->positions || p->max_pos < 1))) return GPTQ_ERR_INVALID;
@@ -68,12 +69,12 @@ int paged_append(const paged_append_t *p, int dtype, void *stream) {
 
 int64_t paged_attention_scratch(const paged_attention_t *p, int dtype) {
 	if (!p || !known(dtype) || p->dim < 1 || p->dim > PAGED_MAX_DIM) return -1;
-	if (!heads_ok(p->heads, p->kv_heads) || p->page < 1) return -1;
+	if (!heads_ok(p->heads, p->kv_heads) || !page_ok(p->page)) return -1;
 	return pg_rows_scratch(*p) + (tiles(*p, dtype) ? pg_tiles_scratch(*p) : 0);
 }
 
 int paged_attention(const paged_attention_t *p, int dtype, void *stream) {
-	if (!p || !known(dtype) || p->requests < 0 || p->requests > PAGED_MAX_REQUESTS || p->rows < 0 || !heads_ok(p->heads, p->kv_heads) || p->page < 1 || p->pages < 0 || p->table_width < 1 ||
+	if (!p || !known(dtype) || p->requests < 0 || p->requests > PAGED_MAX_REQUESTS || p->rows < 0 || !heads_ok(p->heads, p->kv_heads) || !page_ok(p->page) || p->pages < 0 || p->table_width < 1 ||
 		p->table_ld < p->table_width || !(p->scale > 0.f) || !(p->scale <= 3.4e38f) || !p->status)
 		return GPTQ_ERR_INVALID;
 	if (p->dim < 1 || p->dim > PAGED_MAX_DIM || p->dim % 8) return GPTQ_ERR_SHAPE;

@@ -99,7 +99,7 @@ def paged_plan(past: torch.Tensor, new: torch.Tensor, table: torch.Tensor, cache
 	R, rows, heads = past.numel(), int(rows), int(heads)
 	if new.numel() != R or table.shape[0] != R or R > _paged.MAX_REQUESTS:
 		raise ValueError(f'past, new and table must speak of the same requests, at most {_paged.MAX_REQUESTS}: {R}, {new.numel()}, {table.shape[0]}')
-	if rows < 0 or rows >= 1 << 30 or kv_heads < 1 or heads < 1 or heads % kv_heads or page < 1 or dim < 1 or table.shape[1] < 1:
+	if rows < 0 or rows >= 1 << 30 or kv_heads < 1 or heads < 1 or heads % kv_heads or heads > 65535 or not 1 <= page <= _paged.MAX_PAGE or dim < 1 or table.shape[1] < 1:
 		raise ValueError(f'paged_plan: {rows} rows, {heads} heads over {kv_heads} key heads, pages of {page} rows of {dim}, {table.shape[1]} table columns')
 	if R > 1 and table.stride(0) < table.shape[1]:
 		raise ValueError(f'table: rows that overlap (strides {table.stride()})')

@@ -22,6 +22,7 @@ extern "C" {
 
 #define PAGED_MAX_REQUESTS 8192
 #define PAGED_MAX_DIM 256
+#define PAGED_MAX_PAGE (1 << 24)      /* positions count up to 2^30 */
 /* bits of the status word (a run that meets one goes on without touching memory that is not its own) */
 #define PAGED_BAD_INDEX 4              /* a page, position or slot outside the cache or the tables, or a negative length */
 #define PAGED_NO_ROOM 8                /* pages of the pool, columns of the table or rows ran out, or a request has more than max_fresh new tokens */

@@ -286,3 +286,11 @@ def test_rows_that_see_nothing_and_masked_values():
 	out = G.paged_attention(q, k, v, make_plan(s, k))
 	want, _, _ = O.attention(s.parts(big)[0], s.k, s.v, s.table, [0, 20, 21], [20, 41])
 	assert (out.cpu().double() - want).abs().max() <= 1e-4
+
+
+def test_numbers_beyond_the_c_types_are_refused(step):
+	k = step.k.to(DEV)
+	ok = dict(past=step.ints(step.past), new=step.ints(step.new), table=step.ints(step.table), cache=k, rows=step.rows, heads=8)
+	for change in (dict(rows=1 << 30), dict(heads=1 << 16), dict(heads=(1 << 32) + 8)):
+		with pytest.raises(ValueError):
+			G.paged_plan(**{**ok, **change})

@@ -91,3 +91,14 @@ def test_cpu_tensors_are_refused(lib):
 	i = torch.zeros(1, dtype=torch.int32)
 	with pytest.raises(_lib.GptqB200Error, match='CUDA'):
 		paged_plan(i, i, i.view(1, 1), torch.zeros(1, 1, 16, 64, dtype=torch.float16), 1, 1)
+
+
+def test_pages_longer_than_positions_count_are_refused(lib):
+	"""Positions are counted up to 2^30; past + page must stay an int."""
+	from gptq_triton_b200 import _paged
+	page = _paged.MAX_PAGE + 1
+	assert lib.paged_plan(ctypes.byref(_plan(page=page)), 2, None) == -1
+	assert lib.paged_append(ctypes.byref(_append(page=page)), 0, None) == -1
+	assert lib.paged_attention(ctypes.byref(_attention(page=page)), 2, None) == -1
+	assert lib.paged_attention_scratch(ctypes.byref(_attention(page=page)), 2) == -1
+	assert lib.paged_attention_scratch(ctypes.byref(_attention(page=page - 1)), 2) > 0
