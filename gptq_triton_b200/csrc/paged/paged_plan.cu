@@ -134,9 +134,10 @@ __device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, co
 	if (E > PL_NEAR && part > 0) return;                   // (the other entries are in global memory, where part 0 has written them)
 	if (E > PL_NEAR) parts = 1;
 	auto blocks_of = [&](int e) { return e < PL_NEAR ? s_entry[e].blocks : w.entries[kind][e].blocks; };
-	// A share is longer than what a job costs besides its blocks, so that no two slots begin at the same place.  One block of 16 keys beyond
-	// that for few rows (one token of 32 heads behind 100, us: 1 block 7.2, 2 8.0, 4 10.0; behind 2 100 11.7, 11.7, 11.8).
-	const int64_t total = (int64_t)units * p.kv_heads, per = max((total + slots - 1) / slots, (int64_t)((kind ? 2 : 1) + pg_begin(kind)));
+	// A share is longer than what a job costs besides its blocks, so that no two slots begin at the same place, by one block (one token of 32
+	// heads behind 100, us: 1 block 7.2, 2 8.0, 4 10.0; behind 2 100 11.7, 11.7, 11.8; 66 tokens of 28 heads over 4 behind 1 336, tiles: 1 block
+	// 23.3, 2 30.1, 4 34.3).
+	const int64_t total = (int64_t)units * p.kv_heads, per = max((total + slots - 1) / slots, (int64_t)(1 + pg_begin(kind)));
 	int whole = 0;
 	if (kind) {
 		// Whole tiles, the longest first, dealt out to the slots forwards and backwards in turn, unless the longest slot would then work
