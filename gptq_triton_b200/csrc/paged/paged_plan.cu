@@ -13,8 +13,8 @@ namespace {
 
 constexpr int PL_THREADS = 1024;
 
-// sums that stop at a limit (associative for values of at least 0)
-__device__ __forceinline__ int add_to(int a, int b, int limit) { return min(a + b, limit); }
+// sums that stop at a limit (associative for values of 0 .. limit, whose own sum may be beyond an int)
+__device__ __forceinline__ int add_to(int a, int b, int limit) { return a > limit - b ? limit : a + b; }
 constexpr int PL_LIMIT = 1 << 30;
 
 // exclusive scan over the CTA of two values per thread; returns the totals in (ta, tb).  s: 66 ints of shared memory
@@ -102,7 +102,7 @@ __device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, co
 						PgWork w) {
 	const int tid = threadIdx.x, R = p.requests, tile_rows = kind ? PG_TILE : PG_ROWS, keys = kind ? PG_TILE_KEYS : PG_KEYS, group = p.heads / p.kv_heads;
 	const int slots = kind ? PG_TILE_SLOTS : PG_SLOTS;
-	const int E = min(s_tiles[R], w.cap[kind]);
+	int E = min(s_tiles[R], w.cap[kind]);
 	int units = 0;
 	for (int base = 0; base < E; base += PL_THREADS) {
 		const int e = base + tid;
@@ -129,7 +129,10 @@ __device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, co
 		}
 		units = add_to(units, total, PL_LIMIT);
 	}
-	if (units >= PL_LIMIT && tid == 0) atomicOr(p.status, PAGED_NO_ROOM);          // (more keys than the lists count: 10^9 blocks)
+	if (units >= PL_LIMIT) {                               // more keys than the lists count (10^9 blocks): an empty list
+		if (tid == 0) atomicOr(p.status, PAGED_NO_ROOM);
+		E = units = 0;
+	}
 	__syncthreads();
 	if (E > PL_NEAR && part > 0) return;                   // (the other entries are in global memory, where part 0 has written them)
 	if (E > PL_NEAR) parts = 1;
