@@ -44,7 +44,7 @@ int paged_version(void) { return 100; }
 int paged_last_cuda_error(void) { return g_last_cuda_error; }
 
 int64_t paged_work_ints(int requests, int rows, int heads, int kv_heads) {
-	if (requests < 0 || requests > PAGED_MAX_REQUESTS || rows < 0 || !heads_ok(heads, kv_heads) || (int64_t)rows * (heads / kv_heads) >= (int64_t)1 << 31) return -1;
+	if (requests < 0 || requests > PAGED_MAX_REQUESTS || rows < 0 || rows >= 1 << 30 || !heads_ok(heads, kv_heads) || (int64_t)rows * (heads / kv_heads) >= (int64_t)1 << 31) return -1;
 	return pg_work(nullptr, requests, rows, heads, kv_heads).ints;
 }
 
@@ -75,7 +75,7 @@ int64_t paged_attention_scratch(const paged_attention_t *p, int dtype) {
 
 int paged_attention(const paged_attention_t *p, int dtype, void *stream) {
 	if (!p || !known(dtype) || p->requests < 0 || p->requests > PAGED_MAX_REQUESTS || p->rows < 0 || !heads_ok(p->heads, p->kv_heads) || !page_ok(p->page) || p->pages < 0 || p->table_width < 1 ||
-		p->table_ld < p->table_width || !(p->scale > 0.f) || !(p->scale <= 3.4e38f) || !p->status)
+		p->table_ld < p->table_width || !(p->scale > 0.f) || !(p->scale <= 3.4e38f) || !p->status || p->max_fresh < 0 || paged_work_ints(p->requests, p->rows, p->heads, p->kv_heads) < 0)
 		return GPTQ_ERR_INVALID;
 	if (p->dim < 1 || p->dim > PAGED_MAX_DIM || p->dim % 8) return GPTQ_ERR_SHAPE;
 	if (p->requests == 0 || p->rows == 0) return GPTQ_OK;

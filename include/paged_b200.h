@@ -85,7 +85,7 @@ typedef struct {
 
 int paged_version(void);
 int paged_last_cuda_error(void);
-/* int32 values of paged_plan_t.work */
+/* int32 values of paged_plan_t.work; -1: no plan has these sizes (rows below 2^30, rows times query heads of a key head below 2^31) */
 int64_t paged_work_ints(int requests, int rows, int heads, int kv_heads);
 int paged_plan(const paged_plan_t *args, int dtype, void *stream);
 int paged_append(const paged_append_t *args, int dtype, void *stream);
