@@ -1,6 +1,8 @@
 // Joins the partial results of tiles whose keys are spread over several slots of an attention kernel: numerators, maxima (base 2) and sums
-// of a row, in the order of the slots.
+// of a row.
 //   m = max m_i,  l = sum l_i 2^(m_i - m),  out = (sum a_i 2^(m_i - m)) / l
+// The order of the additions is fixed by the sizes alone, so that results repeat bit by bit: a group of lanes (all 32; 16 for heads of up to 64)
+// takes every n-th partial result in the order of the slots, the second half of a warp is added to the first, warp 1, 2 .. to warp 0.
 #include "paged.cuh"
 
 namespace gptq {
@@ -36,7 +38,8 @@ __device__ __forceinline__ Cut read_cut(const PgWork &work, int kind, const PgLi
 }
 
 // A warp adds up ROWS rows from `row0` on of the partial results first, first + step ..; lanes take four columns each, and where a row has
-// fewer than 128 every second (fourth ..) partial result.
+// fewer than 128 every second partial result.  The sum of all is in the first DP / 4 lanes; their partners, which fold the same the other way round,
+// have another rounding of it.
 template <int DP, int ROWS>
 __device__ __forceinline__ void add_up(const Cut &c, int tile_rows, int row0, int rows, const float *scratch, int col0, int first, int step, Sum (&sum)[ROWS]) {
 	constexpr int LANES = DP / 4 < 32 ? DP / 4 : 32, SHARE = 32 / LANES, BATCH = ROWS > 1 ? 2 : 8;
@@ -71,7 +74,7 @@ __device__ __forceinline__ void add_up(const Cut &c, int tile_rows, int row0, in
 		}
 }
 
-template <typename T>
+template <typename T, int DP>
 __device__ __forceinline__ void write(const paged_attention_t &p, const Cut &c, int tile_rows, int row, int col, const Sum &sum) {
 	const int group = p.heads / p.kv_heads;
 	const PgEntry &e = c.s.job;
@@ -79,7 +82,7 @@ __device__ __forceinline__ void write(const paged_attention_t &p, const Cut &c, 
 	const int token = (int)(at / group), head = (int)(at - (int64_t)token * group);
 	const bool blind = e.len - e.fresh + token < 0;          // a row that sees nothing
 	const float f = 1.f / sum.l;
-	if (col < p.dim)
+	if (col < p.dim && (threadIdx.x & 31) < DP / 4)          // (the lanes that hold the sum)
 		store_four<T>(reinterpret_cast<T *>(p.out) + ((int64_t)(e.row + token) * p.heads + c.s.kv * group + head) * p.dim + col,
 					  blind ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.a.x * f, sum.a.y * f, sum.a.z * f, sum.a.w * f));
 }
@@ -122,7 +125,7 @@ __global__ void __launch_bounds__(JN_THREADS, 2) join_kernel(const paged_attenti
 						for (int w = 1; w < JN_WARPS; ++w) fold(sum[0], s_sum[w][lane].m, s_sum[w][lane].l, s_sum[w][lane].a);
 					}
 				}
-				if (!together || warp == 0) write<T>(p, c, PG_ROWS, row, col + 128 * x, sum[0]);
+				if (!together || warp == 0) write<T, DP>(p, c, PG_ROWS, row, col + 128 * x, sum[0]);
 			}
 		}
 		u += together ? gridDim.x : gridDim.x * JN_WARPS;
@@ -144,7 +147,7 @@ __global__ void __launch_bounds__(JN_THREADS, 2) join_kernel(const paged_attenti
 			add_up<DP, ROWS>(d, PG_TILE, row0, rows, tile_scratch, 0, 0, 1, sum);
 #pragma unroll
 			for (int r = 0; r < ROWS; ++r)
-				if (r < rows) write<T>(p, d, PG_TILE, row0 + r, col, sum[r]);
+				if (r < rows) write<T, DP>(p, d, PG_TILE, row0 + r, col, sum[r]);
 		}
 	};
 	// few jobs run through many slots each: more partial results of a row at once; many jobs: more rows

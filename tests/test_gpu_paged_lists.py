@@ -1,5 +1,5 @@
 """Work lists of the paged attention at sizes where the plan forms them in another way: more entries than it keeps in shared memory, more
-blocks of keys than it counts."""
+blocks of keys than it counts; the order in which the partial results of cut jobs are added up."""
 import pytest
 import torch
 
@@ -34,3 +34,25 @@ def test_pages_of_many_long_requests_are_counted():
 	plan = G.paged_plan(torch.zeros_like(new), new, table, cache, 4, 1, pool=pool, head=torch.zeros(1, dtype=torch.int32, device=DEV))
 	assert status() == 8
 	assert plan.head.tolist() == [4] and plan.row_start.tolist() == [0] + [4] * 8 and table[0].tolist() == [0, 1, 2, 3] and (table[1:] == -1).all()
+
+
+@pytest.mark.parametrize('first', [0.3, -0.45])
+def test_partial_results_are_added_in_one_order(first):
+	"""Two partial results of one row, keys 0 .. 15 and 16 .. 47, exact in themselves: equal scores within each (weights of one), values that are whole
+	numbers.  Heads of 64 are folded by two halves of a warp, heads of 72 by one lane after the other; both add the first to the second."""
+	L = 48
+	g = torch.Generator().manual_seed(3)
+	values = torch.randint(-999, 1000, (L, 64), generator=g).float()
+	outs = []
+	for dim in (64, 72):
+		k, v, q = torch.zeros(3, 1, 16, dim), torch.zeros(3, 1, 16, dim), torch.zeros(1, 1, dim)
+		k[0, 0, :, 0] = first
+		q[0, 0, 0] = 1.0
+		v[..., :64] = values.view(3, 1, 16, 64)
+		i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+		k, v, q = k.to(DEV), v.to(DEV), q.to(DEV)
+		plan = G.paged_plan(i32([L - 1]), i32([1]), i32([[0, 1, 2]]), k, 1, 1, max_new=1)
+		outs.append(G.paged_attention(q, k, v, plan, scale=1.0)[0, 0, :64].cpu())
+	w = torch.tensor([first] * 16 + [0.0] * 32, dtype=torch.float64).softmax(0)
+	assert ((outs[0].double() - w @ values.double()).abs() <= 2e-6 * (w @ values.double().abs())).all()
+	assert torch.equal(outs[0], outs[1])
