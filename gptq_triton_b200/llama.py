@@ -222,6 +222,7 @@ class DecodeEngine(StaticEngine):
 		self.ss_mlp = torch.zeros((batch, tiles), dtype=torch.float32, device=dev)
 		self.len_hint = max_seq
 		self._qao_scratch = None
+		self._captured_tables = None
 		self.used_qkv_attn = False          # set when a decode step ran the one-kernel QKV + attention path
 		self.used_fused_oproj = False       # ... with o_proj and the residual add in the same kernel
 		# One persistent kernel per decode step (gptq_decode_chain) + the lm_head / arg-max kernel, where the model
@@ -487,6 +488,8 @@ class DecodeEngine(StaticEngine):
 		self.pos.add_(1)
 
 	def _before_capture(self):
+		# the captured step reads the rotary tables at their addresses, and a call with more positions replaces those of a layer
+		self._captured_tables = [layer.self_attn.tables(self.device, self.max_seq) for layer in self.model.model.layers]
 		if self.ar_o is not None:
 			# the fused exchange waits at most two seconds for a peer: start the ranks together
 			import torch.distributed as dist
@@ -497,6 +500,7 @@ class DecodeEngine(StaticEngine):
 		"""Releases the tensor-parallel exchange buffers (mapped by the peers: call it on every rank, after the
 		last step has completed everywhere) and the captured graph."""
 		super().close()
+		self._captured_tables = None
 		for name in ('ar_o', 'ar_down'):
 			ex = getattr(self, name, None)
 			if ex is not None:
