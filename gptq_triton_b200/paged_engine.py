@@ -15,7 +15,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
-from .fused_attention import QuantLlamaAttention
+from .fused_attention import QuantLlamaAttention, rope_tables
 from .fused_attention import rmsnorm as rmsnorm_kernel
 from ._paged import MAX_REQUESTS
 from .paged import paged_append, paged_attention, paged_plan
@@ -61,7 +61,7 @@ class PagedEngine:
 		zeros = lambda *s, dtype=torch.float16: torch.zeros(s, dtype=dtype, device=self.device)
 		self.kcache = [zeros(*shape) for _ in model.model.layers]
 		self.vcache = [zeros(*shape) for _ in model.model.layers]
-		self.cos, self.sin = attn.tables(self.device, self.max_seq)
+		self.cos, self.sin = rope_tables(self.dim, self.max_seq, attn.rope_theta, device=self.device)          # (those of the layers belong to other engines' captured steps)
 		self.table = zeros(requests, -(-self.max_seq // page_size), dtype=torch.int32)
 		# what a step reads: cached and new tokens per slot, tokens of the rows, free pages in the order in which they are taken
 		self.past, self.new = zeros(requests, dtype=torch.int32), zeros(requests, dtype=torch.int32)
