@@ -74,6 +74,7 @@ class PagedEngine:
 		self.results: Dict[int, List[int]] = {}
 		self._numbers = 0
 		self._graphs: Dict[int, torch.cuda.CUDAGraph] = {}
+		self._stream: Optional[torch.cuda.Stream] = None     # on which decode steps are captured and replayed
 		self._decoding = None                                # the requests that the device buffers are set up for
 
 	# -- requests ------------------------------------------------------------------------------------
@@ -218,26 +219,31 @@ class PagedEngine:
 		if not self.use_graph:
 			self._decode_body(last)
 		else:
-			if last not in self._graphs:
-				self._graphs[last] = self._capture(last)
-			self._graphs[last].replay()
+			# A captured step runs on the stream of its capture: the workspaces of the projections in it belong to that stream, and whoever else
+			# is given the same one (torch deals out 32 per device in turn) is in order with the step.
+			if self._stream is None:
+				self._stream = torch.cuda.Stream(self.device)
+			here, s = torch.cuda.current_stream(self.device), self._stream
+			s.wait_stream(here)
+			with torch.cuda.stream(s):
+				if last not in self._graphs:
+					self._graphs[last] = self._capture(last)
+				self._graphs[last].replay()
+			here.wait_stream(s)
 		return self.tok[:len(active)]
 
 	def _capture(self, last: int):
-		# The trial run writes pages and cache rows that the first real step writes again.
+		"""On the current stream.  The trial run writes pages and cache rows that the first real step writes again."""
 		state = (self.past, self.tok, self.head)
 		saved = [t.clone() for t in state]
-		s = torch.cuda.Stream(self.device)
-		s.wait_stream(torch.cuda.current_stream(self.device))
+		s = torch.cuda.current_stream(self.device)
 		g = torch.cuda.CUDAGraph()
-		with torch.cuda.stream(s):
+		self._decode_body(last)
+		for t, old in zip(state, saved):
+			t.copy_(old)
+		s.synchronize()
+		with torch.cuda.graph(g, stream=s):
 			self._decode_body(last)
-			for t, old in zip(state, saved):
-				t.copy_(old)
-			s.synchronize()
-			with torch.cuda.graph(g, stream=s):
-				self._decode_body(last)
-		torch.cuda.current_stream(self.device).wait_stream(s)
 		return g
 
 	# -- convenience ---------------------------------------------------------------------------------

@@ -1,4 +1,4 @@
-"""What engines on one model share and what not."""
+"""What engines on one model share and what not: rotary tables, streams with their workspaces."""
 import weakref
 
 import pytest
@@ -29,3 +29,53 @@ def test_a_captured_step_holds_the_tables_that_it_reads(model, batch):
 	assert torch.equal(engine.generate(prompt, 6), want)
 	engine.close()
 	assert all(r() is None for r in refs)          # ... and no longer
+
+
+def count_streams(monkeypatch):
+	made = []
+	real = torch.cuda.Stream
+
+	class Counted(real):
+		def __new__(cls, *a, **kw):
+			if 'stream_id' not in kw:          # (not the wrappers of a stream that exists)
+				made.append(1)
+			return real.__new__(real, *a, **kw)
+	monkeypatch.setattr(torch.cuda, 'Stream', Counted)
+	return made
+
+
+def serve(engine, count, steps=3):
+	"""Requests that come one by one, so that 1 .. count run."""
+	numbers = []
+	for i in range(count):
+		numbers.append(engine.add([1 + i, 2, 3], steps + 2 * (count - i)))
+		engine.step()          # its prompt
+		engine.step()          # single tokens of all that run
+	while engine.busy:
+		engine.step()
+	return [engine.results.pop(n) for n in numbers]
+
+
+def test_one_stream_for_all_captured_steps(model, monkeypatch):
+	engine = G.PagedEngine(model, pages=400, requests=12, max_seq=80)
+	made = count_streams(monkeypatch)
+	serve(engine, 12)
+	assert len(made) <= 1
+	engine.close()
+
+
+def test_captured_steps_run_where_they_were_captured(model, monkeypatch):
+	"""The workspace of a captured projection belongs to the stream of the capture: on it the step also runs, ordered with that of the caller."""
+	engine = G.PagedEngine(model, pages=100, requests=2, max_seq=80)
+	seen = {'capture': set(), 'replay': set()}
+	real_graph, real_replay = torch.cuda.graph, torch.cuda.CUDAGraph.replay
+	monkeypatch.setattr(engine, '_decode_body', lambda last, f=engine._decode_body: (seen['capture'].add(torch.cuda.current_stream().cuda_stream), f(last))[1])
+	monkeypatch.setattr(torch.cuda.CUDAGraph, 'replay', lambda self: (seen['replay'].add(torch.cuda.current_stream().cuda_stream), real_replay(self))[1])
+	a = serve(engine, 2)
+	side = torch.cuda.Stream()
+	side.wait_stream(torch.cuda.current_stream())
+	with torch.cuda.stream(side):
+		assert serve(engine, 2) == a
+	torch.cuda.current_stream().wait_stream(side)
+	assert len(seen['replay']) == 1 and seen['replay'] == seen['capture']
+	engine.close()
