@@ -74,6 +74,7 @@ class PagedEngine:
 		self.results: Dict[int, List[int]] = {}
 		self._numbers = 0
 		self._graphs: Dict[int, torch.cuda.CUDAGraph] = {}
+		self._pool = None                                    # their memory, shared: none needs its own while another runs
 		self._stream: Optional[torch.cuda.Stream] = None     # on which decode steps are captured and replayed
 		self._decoding = None                                # the requests that the device buffers are set up for
 
@@ -207,9 +208,15 @@ class PagedEngine:
 		self.tok[:last].copy_(tok)
 		self.head.copy_(plan.head)                           # (behind the plan's own reading of it)
 
+	def _slots_served(self, last: int) -> int:
+		"""Slots (rows) of a decode step for `last` of them: a few sizes, so that few steps are captured.  Every one up to 8, then four per power of
+		two; the slots behind have no new tokens."""
+		step = (1 << (last - 1).bit_length()) // 8 if last > 8 else 1
+		return min(-(-last // step) * step, len(self.slots))
+
 	def _decode(self, active) -> torch.Tensor:
 		"""A step of single tokens; as long as the same requests run, the device buffers carry on by themselves."""
-		last = max(r.slot for r, _ in active) + 1
+		last = self._slots_served(max(r.slot for r, _ in active) + 1)
 		running = [r.number for r, _ in active]
 		if self._decoding != running:
 			self._upload(active, last)
@@ -238,11 +245,13 @@ class PagedEngine:
 		saved = [t.clone() for t in state]
 		s = torch.cuda.current_stream(self.device)
 		g = torch.cuda.CUDAGraph()
+		if self._pool is None:
+			self._pool = torch.cuda.graph_pool_handle()
 		self._decode_body(last)
 		for t, old in zip(state, saved):
 			t.copy_(old)
 		s.synchronize()
-		with torch.cuda.graph(g, stream=s):
+		with torch.cuda.graph(g, stream=s, pool=self._pool):          # (one at a time is replayed, and what a step leaves lies outside)
 			self._decode_body(last)
 		return g
 
@@ -266,5 +275,6 @@ class PagedEngine:
 		return [self.results.pop(n) for n in numbers]
 
 	def close(self):
-		"""Releases the captured graphs."""
+		"""Releases the captured graphs and their memory."""
 		self._graphs.clear()
+		self._pool = None

@@ -1,4 +1,4 @@
-"""What engines on one model share and what not: rotary tables, streams with their workspaces."""
+"""What engines on one model share and what not: rotary tables, streams with their workspaces, captured steps."""
 import weakref
 
 import pytest
@@ -79,3 +79,14 @@ def test_captured_steps_run_where_they_were_captured(model, monkeypatch):
 	torch.cuda.current_stream().wait_stream(side)
 	assert len(seen['replay']) == 1 and seen['replay'] == seen['capture']
 	engine.close()
+
+
+def test_few_captured_steps_with_one_pool(model):
+	engine = G.PagedEngine(model, pages=2000, requests=40, max_seq=120)
+	with_graph = serve(engine, 40)
+	graphs = list(engine._graphs.values())
+	assert len(graphs) <= 20 and len({g.pool() for g in graphs}) == 1
+	engine.close()
+	assert not engine._graphs
+	assert serve(engine, 3) == serve(G.PagedEngine(model, pages=100, requests=3, max_seq=120, use_graph=False), 3)          # (captured again)
+	assert serve(G.PagedEngine(model, pages=2000, requests=40, max_seq=120, use_graph=False), 40) == with_graph
