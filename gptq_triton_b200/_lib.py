@@ -227,7 +227,8 @@ def kernel_status(device=None) -> int:
 	1 = a TMA / bulk load never completed within the bounded wait; 2 = shared memory misaligned;
 	3 = a wait inside the tensor-core kernel ran out; 4 = position outside the rotary table / cache, or token outside the vocabulary;
 	5 = a peer never arrived in the fused tensor-parallel all-reduce; 6 = a split-K partial sum never arrived;
-	7 = a grid barrier of the persistent decode-step kernel timed out; 8 = pages, table columns or rows of a paged step ran out, or a request had more new tokens than announced)."""
+	7 = a grid barrier of the persistent decode-step kernel timed out; 8 = pages, table columns or rows of a paged step ran out, a request had more new tokens than announced, or its work lists count too few
+	blocks; 16 = a wait inside the paged attention ran out: 4, 8 and 16 are bits that the paged operators set beside one another)."""
 	st = 0
 	for (dev, _), ws in _workspaces.items():
 		if device is None or dev == (device.index if isinstance(device, torch.device) else device):

@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) tiles_kernel(const __grid_const
 	}
 	auto fail = [&]() {
 		*stop = 1;
-		atomicOr(p.status, 3);
+		atomicOr(p.status, PAGED_TIMED_OUT);
 	};
 
 	if (warp >= 8) {

@@ -23,10 +23,11 @@ extern "C" {
 #define PAGED_MAX_REQUESTS 8192
 #define PAGED_MAX_DIM 256
 #define PAGED_MAX_PAGE (1 << 24)      /* positions count up to 2^30 */
-/* bits of the status word (a run that meets one goes on without touching memory that is not its own) */
+/* bits of the status word, none of them a code of gptq_b200.h with another meaning (a run that meets one goes on without touching memory that is not its own) */
 #define PAGED_BAD_INDEX 4              /* a page, position or slot outside the cache or the tables, or a negative length */
 #define PAGED_NO_ROOM 8                /* pages of the pool, columns of the table or rows ran out, or a request has more than max_fresh new tokens; or the
                                           requests see more keys than the work lists count (2^30 blocks of 16): the attention then computes nothing */
+#define PAGED_TIMED_OUT 16             /* a wait inside the attention's kernel for chunks ran out */
 
 /* The plan of one step.  Request r has past[r] tokens in the cache and gets fresh[r] new ones (0 is allowed).  Rows are the new
  * tokens, request after request; rows behind the last one get slot -1 and position 0.
