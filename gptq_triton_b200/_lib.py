@@ -230,14 +230,47 @@ def kernel_status(device=None) -> int:
 	7 = a grid barrier of the persistent decode-step kernel timed out; 8 = pages, table columns or rows of a paged step ran out, a request had more new tokens than announced, or its work lists count too few
 	blocks; 16 = a wait inside the paged attention ran out: 4, 8 and 16 are bits that the paged operators set beside one another)."""
 	st = 0
-	for (dev, _), ws in _workspaces.items():
+	for (dev, _), ws in list(_workspaces.items()):
 		if device is None or dev == (device.index if isinstance(device, torch.device) else device):
-			st |= int(ws[16384 - 4:16384].view(torch.int32).item())
+			st |= int(status_word(ws).item())
 	for ref in _status_buffers:
 		buf = ref()
 		if buf is not None and (device is None or buf.device.index == (device.index if isinstance(device, torch.device) else device)):
-			st |= int(buf[16384 - 4:16384].view(torch.int32).item())
+			st |= int(status_word(buf).item())
 	return st
+
+
+def status_word(buf: torch.Tensor) -> torch.Tensor:
+	"""The word of one buffer that kernel_status() reads, int32 [1] on its device."""
+	return buf[16384 - 4:16384].view(torch.int32)
+
+
+class OwnWorkspace:
+	"""Within `with`, layers on the current stream of `device` work in a buffer that this object keeps, not in the one of the stream.  For a capture: what
+	is captured there may then be replayed on any stream and shares its workspace with no other work, whoever is given the stream of the capture
+	next (torch deals out 32 per device in turn)."""
+
+	def __init__(self, device: torch.device):
+		self.index = device.index if device.index is not None else torch.cuda.current_device()
+		self.buffer: Optional[torch.Tensor] = None
+		self.older = []          # smaller ones, which earlier captures read
+
+	def __enter__(self):
+		self.key = (self.index, _raw_stream(self.index))
+		self.streams = _workspaces.pop(self.key, None)
+		if self.buffer is not None:
+			_workspaces[self.key] = self.buffer
+
+	def __exit__(self, *e):
+		mine = _workspaces.pop(self.key, None)
+		if mine is not self.buffer:          # the first one, or a larger one
+			self.older += [buf for buf in _retired if buf is self.buffer]
+			_retired[:] = [buf for buf in _retired if buf is not self.buffer]
+			self.buffer = mine
+			register_status_buffer(mine)
+		if self.streams is not None:
+			_workspaces[self.key] = self.streams
+		self.streams = None
 
 
 def clear_kernel_status():

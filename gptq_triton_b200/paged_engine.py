@@ -15,9 +15,9 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from . import _lib, _paged
 from .fused_attention import QuantLlamaAttention, rope_tables
 from .fused_attention import rmsnorm as rmsnorm_kernel
-from ._paged import MAX_REQUESTS
 from .paged import paged_append, paged_attention, paged_plan
 
 
@@ -49,7 +49,7 @@ class PagedEngine:
 		for layer in model.model.layers:
 			if not isinstance(layer.self_attn, QuantLlamaAttention):
 				raise ValueError('PagedEngine: run make_quant_attn first')
-		if pages < 1 or page_size < 1 or not 1 <= requests <= MAX_REQUESTS or portion < 1:
+		if pages < 1 or page_size < 1 or not 1 <= requests <= _paged.MAX_REQUESTS or portion < 1:
 			raise ValueError(f'PagedEngine: {pages} pages of {page_size}, {requests} requests, portions of {portion}')
 		self.model, self.cfg = model, model.config
 		self.device = model.lm_head.weight.device
@@ -74,8 +74,8 @@ class PagedEngine:
 		self.results: Dict[int, List[int]] = {}
 		self._numbers = 0
 		self._graphs: Dict[int, torch.cuda.CUDAGraph] = {}
-		self._pool = None                                    # their memory, shared: none needs its own while another runs
-		self._stream: Optional[torch.cuda.Stream] = None     # on which decode steps are captured and replayed
+		# of all captures: their stream, the workspace of their projections, their memory (none needs its own while another runs)
+		self._stream = self._workspace = self._pool = None
 		self._decoding = None                                # the requests that the device buffers are set up for
 
 	# -- requests ------------------------------------------------------------------------------------
@@ -225,41 +225,35 @@ class PagedEngine:
 			self._decoding = running
 		if not self.use_graph:
 			self._decode_body(last)
-		else:
-			# A captured step runs on the stream of its capture: the workspaces of the projections in it belong to that stream, and whoever else
-			# is given the same one (torch deals out 32 per device in turn) is in order with the step.
-			if self._stream is None:
-				self._stream = torch.cuda.Stream(self.device)
-			here, s = torch.cuda.current_stream(self.device), self._stream
-			s.wait_stream(here)
-			with torch.cuda.stream(s):
-				if last not in self._graphs:
-					self._graphs[last] = self._capture(last)
-				self._graphs[last].replay()
-			here.wait_stream(s)
+			return self.tok[:len(active)]
+		if last not in self._graphs:
+			self._graphs[last] = self._capture(last)
+		self._graphs[last].replay()
 		return self.tok[:len(active)]
 
-	def _capture(self, last: int):
-		"""On the current stream.  The trial run writes pages and cache rows that the first real step writes again."""
+	def _capture(self, last: int) -> torch.cuda.CUDAGraph:
+		# The trial run writes pages and cache rows that the first real step writes again.
+		if self._stream is None:
+			self._stream, self._workspace, self._pool = torch.cuda.Stream(self.device), _lib.OwnWorkspace(self.device), torch.cuda.graph_pool_handle()
+		here, s = torch.cuda.current_stream(self.device), self._stream
 		state = (self.past, self.tok, self.head)
 		saved = [t.clone() for t in state]
-		s = torch.cuda.current_stream(self.device)
+		s.wait_stream(here)
 		g = torch.cuda.CUDAGraph()
-		if self._pool is None:
-			self._pool = torch.cuda.graph_pool_handle()
-		self._decode_body(last)
-		for t, old in zip(state, saved):
-			t.copy_(old)
-		s.synchronize()
-		with torch.cuda.graph(g, stream=s, pool=self._pool):          # (one at a time is replayed, and what a step leaves lies outside)
+		with torch.cuda.stream(s), self._workspace:
 			self._decode_body(last)
+			for t, old in zip(state, saved):
+				t.copy_(old)
+			s.synchronize()
+			with torch.cuda.graph(g, stream=s, pool=self._pool):          # (one at a time is replayed, and what a step leaves lies outside)
+				self._decode_body(last)
+		here.wait_stream(s)
 		return g
 
 	# -- convenience ---------------------------------------------------------------------------------
 	@torch.no_grad()
 	def generate(self, prompts: Sequence[Sequence[int]], steps: int, stop: Optional[int] = None) -> List[List[int]]:
 		"""Greedy generation for prompts of any lengths: the generated tokens of each."""
-		from . import _lib
 		numbers = []
 		try:
 			for p in prompts:
@@ -277,4 +271,4 @@ class PagedEngine:
 	def close(self):
 		"""Releases the captured graphs and their memory."""
 		self._graphs.clear()
-		self._pool = None
+		self._stream = self._workspace = self._pool = None

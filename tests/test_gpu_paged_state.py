@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import gptq_triton_b200 as G
+from gptq_triton_b200 import _lib
 from test_gpu_decode import build_pair
 
 pytestmark = pytest.mark.gpu
@@ -64,21 +65,33 @@ def test_one_stream_for_all_captured_steps(model, monkeypatch):
 	engine.close()
 
 
-def test_captured_steps_run_where_they_were_captured(model, monkeypatch):
-	"""The workspace of a captured projection belongs to the stream of the capture: on it the step also runs, ordered with that of the caller."""
-	engine = G.PagedEngine(model, pages=100, requests=2, max_seq=80)
-	seen = {'capture': set(), 'replay': set()}
-	real_graph, real_replay = torch.cuda.graph, torch.cuda.CUDAGraph.replay
-	monkeypatch.setattr(engine, '_decode_body', lambda last, f=engine._decode_body: (seen['capture'].add(torch.cuda.current_stream().cuda_stream), f(last))[1])
-	monkeypatch.setattr(torch.cuda.CUDAGraph, 'replay', lambda self: (seen['replay'].add(torch.cuda.current_stream().cuda_stream), real_replay(self))[1])
-	a = serve(engine, 2)
+def test_captured_steps_share_their_workspace_with_nobody(model):
+	"""The workspace of the projections in a captured step is the engine's: no stream has it, that of the capture least of all, whose number somebody
+	else may be given.  Its status word is asked for, and it goes with the engine."""
+	first, second = (G.PagedEngine(model, pages=100, requests=2, max_seq=80) for _ in range(2))
+	want = serve(first, 2)
+	known = dict(_lib._workspaces)
+	assert serve(second, 2) == want and _lib._workspaces.keys() == known.keys()
+	mine = [e._workspace.buffer for e in (first, second)]
+	assert all(m.numel() > 0 and m is not ws for m in mine for ws in [*_lib._workspaces.values(), *_lib._retired]) and mine[0] is not mine[1]
+	_lib.status_word(mine[1]).fill_(3)
+	try:
+		assert _lib.kernel_status() == 3
+		assert serve(first, 2) == want
+	finally:
+		_lib.clear_kernel_status()
 	side = torch.cuda.Stream()
+	with torch.cuda.stream(first._stream):          # the same stream for other work: it has a workspace of its own
+		assert serve(G.PagedEngine(model, pages=100, requests=2, max_seq=80, use_graph=False), 2) == want
 	side.wait_stream(torch.cuda.current_stream())
 	with torch.cuda.stream(side):
-		assert serve(engine, 2) == a
-	torch.cuda.current_stream().wait_stream(side)
-	assert len(seen['replay']) == 1 and seen['replay'] == seen['capture']
-	engine.close()
+		assert serve(first, 2) == want
+	side.synchronize()
+	assert first._workspace.buffer is mine[0]
+	seen = weakref.ref(mine[0])
+	first.close()
+	del mine, first
+	assert seen() is None
 
 
 def test_few_captured_steps_with_one_pool(model):
