@@ -6,6 +6,7 @@ pages given back when a request ends.
 	while engine.busy:
 		for request, token in engine.step():      # one step of all requests that run
 			...
+	tokens = engine.results.pop(a)               # all tokens of a request that has ended; they stay until somebody takes them
 or engine.generate(prompts, steps).  Decoding is greedy.
 """
 from __future__ import annotations
@@ -73,7 +74,8 @@ class PagedEngine:
 		self.waiting: List[_Request] = []
 		self.results: Dict[int, List[int]] = {}
 		self._numbers = 0
-		self._graphs: Dict[int, torch.cuda.CUDAGraph] = {}
+		self.told = zeros(requests + 2, dtype=torch.int32)   # what a step answers: see _tell
+		self._graphs: Dict[int, Tuple[torch.cuda.CUDAGraph, torch.Tensor]] = {}
 		# of all captures: their stream, the workspace of their projections, their memory (none needs its own while another runs)
 		self._stream = self._workspace = self._pool = None
 		self._decoding = None                                # the requests that the device buffers are set up for
@@ -119,11 +121,21 @@ class PagedEngine:
 		self.slots[r.slot] = None
 		self.results[r.number] = r.out
 
+	def _forget(self, numbers: Sequence[int]):
+		self.waiting = [r for r in self.waiting if r.number not in numbers]
+		for r in self.slots:
+			if r is not None and r.number in numbers:
+				self._finish(r)
+		self._decoding = None
+		for n in numbers:
+			self.results.pop(n, None)
+
 	# -- a step --------------------------------------------------------------------------------------
 	@torch.no_grad()
 	def step(self) -> List[Tuple[int, int]]:
 		"""One step: every running request feeds its next token or a portion of its prompt.  Returns (request, token) for those that have
-		generated one."""
+		generated one.  Raises when a kernel has reported a status (see _lib.kernel_status): that step gives no tokens, and the
+		requests that took part in it end without results."""
 		self._admit()
 		running = [r for r in self.slots if r is not None]
 		if not running:
@@ -137,14 +149,17 @@ class PagedEngine:
 			feed.append(n)
 		active = [(r, n) for r, n in zip(running, feed) if n]
 		decode = all(r.pending == 1 and n == 1 for r, n in zip(running, feed))
-		logits_rows = self._decode(active) if decode else self._mixed(active)
+		try:
+			tokens = self._decode(active) if decode else self._mixed(active)
+		except _lib.GptqB200Error:
+			self._forget([r.number for r, _ in active])
+			raise
 		for r, n in active:
 			taken = self._needs(r.fed + n) - len(r.pages)
 			r.pages += self.free[:taken]
 			del self.free[:taken]
 			self.reserved -= taken
 			r.fed += n
-		tokens = logits_rows.tolist()                        # (waits for the device)
 		done = []
 		for (r, n), t in zip(active, tokens):
 			if r.fed < len(r.prompt):
@@ -155,6 +170,21 @@ class PagedEngine:
 				self._finish(r)
 				self._decoding = None
 		return done
+
+	def _tell(self, tokens: torch.Tensor) -> torch.Tensor:
+		"""Tokens, and behind them the status words of the layers and of the paged operators: int32 [rows + words]."""
+		index = self.device.index
+		words = [_lib.status_word(buf) for buf in (_lib._workspaces.get((index, _lib.stream_ptr(self.device))), _paged._control.get(index)) if buf is not None]
+		return torch.cat([tokens.to(torch.int32), *words], out=self.told[:len(tokens) + len(words)])
+
+	def _read(self, told: torch.Tensor, rows: int) -> List[int]:
+		values = told.tolist()                                # (waits for the device)
+		status = 0
+		for v in values[rows:]:
+			status |= v
+		if status != 0:
+			raise _lib.GptqB200Error(f'a kernel reported status {status} (see _lib.kernel_status)')
+		return values[:rows]
 
 	def _upload(self, active, last: int):
 		"""Lengths of the slots 0 .. last - 1 and the pages that the step takes."""
@@ -187,7 +217,7 @@ class PagedEngine:
 		norm = self.model.model.norm
 		return self.model.lm_head(rmsnorm_kernel(h.contiguous(), norm.weight, norm.variance_epsilon)).argmax(-1)
 
-	def _mixed(self, active) -> torch.Tensor:
+	def _mixed(self, active) -> List[int]:
 		"""A step with portions of prompts."""
 		last = max(r.slot for r, _ in active) + 1
 		self._upload(active, last)
@@ -199,14 +229,15 @@ class PagedEngine:
 			ends.append(len(ids) - 1)
 		both = torch.tensor(ids + ends, dtype=torch.int64).pin_memory().to(self.device, non_blocking=True)
 		h = self._layers(both[:len(ids)], self._plan(last, len(ids), max(n for _, n in active)))
-		return self._greedy(h.index_select(0, both[len(ids):]))
+		return self._read(self._tell(self._greedy(h.index_select(0, both[len(ids):]))), len(active))
 
-	def _decode_body(self, last: int):
+	def _decode_body(self, last: int) -> torch.Tensor:
 		plan = self._plan(last, last, 1)
 		self.past[:last] += self.new[:last]
 		tok = self._greedy(self._layers(self.tok[:last], plan))
 		self.tok[:last].copy_(tok)
 		self.head.copy_(plan.head)                           # (behind the plan's own reading of it)
+		return self._tell(tok)
 
 	def _slots_served(self, last: int) -> int:
 		"""Slots (rows) of a decode step for `last` of them: a few sizes, so that few steps are captured.  Every one up to 8, then four per power of
@@ -214,7 +245,7 @@ class PagedEngine:
 		step = (1 << (last - 1).bit_length()) // 8 if last > 8 else 1
 		return min(-(-last // step) * step, len(self.slots))
 
-	def _decode(self, active) -> torch.Tensor:
+	def _decode(self, active) -> List[int]:
 		"""A step of single tokens; as long as the same requests run, the device buffers carry on by themselves."""
 		last = self._slots_served(max(r.slot for r, _ in active) + 1)
 		running = [r.number for r, _ in active]
@@ -224,14 +255,14 @@ class PagedEngine:
 			self.tok[:len(active)] = torch.tensor(known, dtype=torch.int64).pin_memory().to(self.device, non_blocking=True)
 			self._decoding = running
 		if not self.use_graph:
-			self._decode_body(last)
-			return self.tok[:len(active)]
+			return self._read(self._decode_body(last), last)[:len(active)]
 		if last not in self._graphs:
 			self._graphs[last] = self._capture(last)
-		self._graphs[last].replay()
-		return self.tok[:len(active)]
+		graph, told = self._graphs[last]
+		graph.replay()
+		return self._read(told, last)[:len(active)]
 
-	def _capture(self, last: int) -> torch.cuda.CUDAGraph:
+	def _capture(self, last: int) -> Tuple[torch.cuda.CUDAGraph, torch.Tensor]:
 		# The trial run writes pages and cache rows that the first real step writes again.
 		if self._stream is None:
 			self._stream, self._workspace, self._pool = torch.cuda.Stream(self.device), _lib.OwnWorkspace(self.device), torch.cuda.graph_pool_handle()
@@ -246,9 +277,9 @@ class PagedEngine:
 				t.copy_(old)
 			s.synchronize()
 			with torch.cuda.graph(g, stream=s, pool=self._pool):          # (one at a time is replayed, and what a step leaves lies outside)
-				self._decode_body(last)
+				told = self._decode_body(last)
 		here.wait_stream(s)
-		return g
+		return g, told
 
 	# -- convenience ---------------------------------------------------------------------------------
 	@torch.no_grad()
@@ -258,14 +289,14 @@ class PagedEngine:
 		try:
 			for p in prompts:
 				numbers.append(self.add(p, steps, stop))
-		except Exception:                                     # one is refused: none of them stays queued
-			self.waiting = [r for r in self.waiting if r.number not in numbers]
+			while self.busy:
+				self.step()
+			status = _lib.kernel_status(self.device)
+			if status != 0:
+				raise _lib.GptqB200Error(f'a kernel reported status {status} (see _lib.kernel_status)')
+		except Exception:                                     # a prompt is refused, or a step has failed: none of them stays
+			self._forget(numbers)
 			raise
-		while self.busy:
-			self.step()
-		status = _lib.kernel_status(self.device)
-		if status != 0:
-			raise _lib.GptqB200Error(f'a kernel reported status {status} (see _lib.kernel_status)')
 		return [self.results.pop(n) for n in numbers]
 
 	def close(self):

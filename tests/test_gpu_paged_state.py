@@ -1,11 +1,12 @@
-"""What engines on one model share and what not: rotary tables, streams with their workspaces, captured steps."""
+"""What engines on one model share and what not: rotary tables, streams with their workspaces, captured steps; status words that a
+step meets."""
 import weakref
 
 import pytest
 import torch
 
 import gptq_triton_b200 as G
-from gptq_triton_b200 import _lib
+from gptq_triton_b200 import _lib, _paged
 from test_gpu_decode import build_pair
 
 pytestmark = pytest.mark.gpu
@@ -78,6 +79,8 @@ def test_captured_steps_share_their_workspace_with_nobody(model):
 	try:
 		assert _lib.kernel_status() == 3
 		assert serve(first, 2) == want
+		with pytest.raises(_lib.GptqB200Error, match='3'):
+			serve(second, 2)
 	finally:
 		_lib.clear_kernel_status()
 	side = torch.cuda.Stream()
@@ -97,9 +100,32 @@ def test_captured_steps_share_their_workspace_with_nobody(model):
 def test_few_captured_steps_with_one_pool(model):
 	engine = G.PagedEngine(model, pages=2000, requests=40, max_seq=120)
 	with_graph = serve(engine, 40)
-	graphs = list(engine._graphs.values())
+	graphs = [g for g, _ in engine._graphs.values()]
 	assert len(graphs) <= 20 and len({g.pool() for g in graphs}) == 1
 	engine.close()
 	assert not engine._graphs
 	assert serve(engine, 3) == serve(G.PagedEngine(model, pages=100, requests=3, max_seq=120, use_graph=False), 3)          # (captured again)
 	assert serve(G.PagedEngine(model, pages=2000, requests=40, max_seq=120, use_graph=False), 40) == with_graph
+
+
+def test_a_step_that_meets_a_status_raises(model):
+	engine = G.PagedEngine(model, pages=40, requests=2, max_seq=80)
+	a = engine.add([1, 2, 3], 6)
+	engine.step()
+	engine.step()
+	b = engine.add([4], 3)
+	word = _paged._control[0][_paged.CONTROL_BYTES - 4:].view(torch.int32)
+	word.fill_(8)
+	try:
+		with pytest.raises(_lib.GptqB200Error, match='8'):
+			engine.step()
+		assert not engine.busy and sorted(engine.free) == list(range(40)) and engine.reserved == 0 and not engine.results
+		with pytest.raises(_lib.GptqB200Error, match='8'):
+			engine.generate([[1, 2], [3], [4, 5, 6]], 4)
+		assert not engine.busy and sorted(engine.free) == list(range(40)) and engine.reserved == 0 and not engine.results
+	finally:
+		_lib.clear_kernel_status()
+	c = engine.add([1, 2, 3], 6)
+	while engine.busy:
+		engine.step()
+	assert len(engine.results.pop(c)) == 6 and a < b < c
