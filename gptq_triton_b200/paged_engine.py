@@ -140,15 +140,15 @@ class PagedEngine:
 		running = [r for r in self.slots if r is not None]
 		if not running:
 			return []
-		left, feed = self.portion, []
-		for r in running:                                    # single tokens always go on; portions share what a step may take
+		left, feed = self.portion, {}
+		for r in sorted(running, key=lambda r: r.number):    # single tokens always go on; portions share what a step may take, the first request first
 			n = r.pending
 			if n > 1:
 				n = min(n, left)
 				left -= n
-			feed.append(n)
-		active = [(r, n) for r, n in zip(running, feed) if n]
-		decode = all(r.pending == 1 and n == 1 for r, n in zip(running, feed))
+			feed[r.number] = n
+		active = [(r, feed[r.number]) for r in running if feed[r.number]]          # (rows in the order of the slots)
+		decode = all(r.pending == 1 for r in running)
 		try:
 			tokens = self._decode(active) if decode else self._mixed(active)
 		except _lib.GptqB200Error:
