@@ -13,8 +13,8 @@ namespace {
 
 constexpr int PL_THREADS = 1024;
 
-// sums that stop at a limit (associative for values of 0 .. limit, whose own sum may be beyond an int)
-__device__ __forceinline__ int add_to(int a, int b, int limit) { return a > limit - b ? limit : a + b; }
+// sums that stop at a limit (associative for values of 0 .. limit; the sum of two limits of 2^30 is beyond an int)
+__device__ __forceinline__ int add_to(int a, int b, int limit) { return (int)min((unsigned)a + (unsigned)b, (unsigned)limit); }
 constexpr int PL_LIMIT = 1 << 30;
 
 // exclusive scan over the CTA of two values per thread; returns the totals in (ta, tb).  s: 66 ints of shared memory
@@ -129,10 +129,10 @@ __device__ void lay_out(const paged_plan_t &p, int kind, int part, int parts, co
 		}
 		units = add_to(units, total, PL_LIMIT);
 	}
-	if (units >= PL_LIMIT) {                               // more keys than the lists count (10^9 blocks): an empty list
-		if (tid == 0) atomicOr(p.status, PAGED_NO_ROOM);
-		E = units = 0;
-	}
+	const bool over = units >= PL_LIMIT;                   // more keys than the lists count (10^9 blocks): an empty list
+	if (over && tid == 0) atomicOr(p.status, PAGED_NO_ROOM);
+	E = over ? 0 : E;
+	units = over ? 0 : units;
 	__syncthreads();
 	if (E > PL_NEAR && part > 0) return;                   // (the other entries are in global memory, where part 0 has written them)
 	if (E > PL_NEAR) parts = 1;
