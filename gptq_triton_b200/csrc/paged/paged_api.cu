@@ -33,6 +33,12 @@ bool page_ok(int page) { return page >= 1 && page <= PAGED_MAX_PAGE; }
 bool heads_ok(int heads, int kv_heads) { return kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && heads <= 65535; }
 // heads and pages start on 16 bytes
 bool steps_ok(int64_t a, int64_t b, int dtype) { return a * size_of(dtype) % 16 == 0 && b * size_of(dtype) % 16 == 0; }
+// pages, and key heads within them, are places of their own
+template <typename P>
+bool places_ok(const P &p) {
+	const int64_t least = (int64_t)p.page * p.dim;
+	return !(p.pages > 1 && (p.k_page < least || p.v_page < least)) && !(p.kv_heads > 1 && (p.k_kv < least || p.v_kv < least));
+}
 
 bool tiles(const paged_attention_t &p, int dtype) { return p.pages > 0 && pg_tiles_serve(dtype, p.dim, p.page, p.max_fresh, p.heads, p.kv_heads); }
 
@@ -63,7 +69,8 @@ int paged_append(const paged_append_t *p, int dtype, void *stream) {
 	if (!p || !known(dtype) || p->rows < 0 || !heads_ok(p->heads, p->kv_heads) || p->dim < 1 || p->rot < 0 || p->rot > p->dim || p->rot % 2 || !page_ok(p->page) || p->pages < 0 || !p->status)
 		return GPTQ_ERR_INVALID;
 	if (p->rows == 0) return GPTQ_OK;
-	if (!p->q || !p->k || !p->v || !p->q_out || !p->k_cache || !p->v_cache || !p->slots || (p->rot && (!p->cos_t || !p->sin_t || !p->positions || p->max_pos < 1))) return GPTQ_ERR_INVALID;
+	if (!p->q || !p->k || !p->v || !p->q_out || !p->k_cache || !p->v_cache || !p->slots || (p->rot && (!p->cos_t || !p->sin_t || !p->positions || p->max_pos < 1)) || !places_ok(*p))
+		return GPTQ_ERR_INVALID;
 	return pg_append_launch(*p, dtype, (cudaStream_t)stream);
 }
 
@@ -80,12 +87,7 @@ int paged_attention(const paged_attention_t *p, int dtype, void *stream) {
 	if (p->dim < 1 || p->dim > PAGED_MAX_DIM || p->dim % 8) return GPTQ_ERR_SHAPE;
 	if (p->requests == 0 || p->rows == 0) return GPTQ_OK;
 	if (!p->q || !p->k_cache || !p->v_cache || !p->table || !p->row_start || !p->lens || !p->work || !p->out) return GPTQ_ERR_INVALID;
-	// pages, and key heads within them, are places of their own
-	const int64_t least = (int64_t)p->page * p->dim;
-	for (int64_t s : {p->k_page, p->v_page})
-		if (p->pages > 1 && s < least) return GPTQ_ERR_INVALID;
-	for (int64_t s : {p->k_kv, p->v_kv})
-		if (p->kv_heads > 1 && s < least) return GPTQ_ERR_INVALID;
+	if (!places_ok(*p)) return GPTQ_ERR_INVALID;
 	if (!steps_ok(p->k_page, p->k_kv, dtype) || !steps_ok(p->v_page, p->v_kv, dtype) || !steps_ok(p->q_row, p->q_head, dtype) || !aligned16(p->q) || !aligned16(p->k_cache) || !aligned16(p->v_cache) ||
 		!aligned16(p->out))
 		return GPTQ_ERR_ALIGN;

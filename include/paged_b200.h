@@ -63,11 +63,12 @@ typedef struct {
 	const int64_t *slots;
 	void *q_out;                       /* [rows, heads, dim] contiguous */
 	void *k_cache, *v_cache;
-	int64_t k_page, k_kv, v_page, v_kv;                            /* strides of pages and heads in elements */
+	int64_t k_page, k_kv, v_page, v_kv;                            /* strides of pages and heads in elements, a page's rows (page * dim) at least */
 	int *status;
 } paged_append_t;
 
-/* out[row] = softmax over positions 0 .. p of scale * q . k, times v; p = position of the row.  Rows that belong to no request
+/* table, row_start, lens and work are those of a plan of the same requests, rows, heads, kv_heads, dim, page, pages, table_width, max_fresh and dtype.
+ * out[row] = softmax over positions 0 .. p of scale * q . k, times v; p = position of the row.  Rows that belong to no request
  * (behind the last one) are left as they are. */
 typedef struct {
 	int requests, rows, heads, kv_heads, dim, page, pages, table_width, max_fresh;

@@ -6,7 +6,7 @@ from pathlib import Path
 
 import pytest
 
-from test_paged_cpu import _attention, _plan, lib      # noqa: F401
+from test_paged_cpu import _append, _attention, _plan, lib      # noqa: F401
 
 
 @pytest.mark.parametrize('sizes', [dict(rows=1 << 30, heads=1, kv_heads=1), dict(rows=2 ** 31 - 1, heads=1, kv_heads=1), dict(rows=1 << 20, heads=4096, kv_heads=1)], ids=str)
@@ -30,3 +30,10 @@ def test_status_bits():
 	for f in (root / 'gptq_triton_b200' / 'csrc' / 'paged').glob('*.cu'):
 		for what in re.findall(r'atomicOr\(p\.status, ([^)]*)\)', f.read_text()):
 			assert what in (*bits, 'bad'), (f.name, what)
+
+
+@pytest.mark.parametrize('kw', [dict(k_page=0), dict(v_page=1023), dict(k_kv=0), dict(v_kv=1023)], ids=str)
+def test_append_refuses_pages_that_lie_on_one_another(lib, kw):          # noqa: F811
+	strides = dict(q_row=256, q_head=64, k_row=128, k_head=64, v_row=128, v_head=64, k_page=2048, k_kv=1024, v_page=2048, v_kv=1024)
+	assert lib.paged_append(ctypes.byref(_append(**{**strides, **kw})), 2, None) == -1
+	assert lib.paged_append(ctypes.byref(_append(**{**strides, **kw, 'rows': 0})), 2, None) == 0
