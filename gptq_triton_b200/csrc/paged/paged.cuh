@@ -38,9 +38,10 @@ template <> struct PgElem<__half> {
 // into equal lengths for the slots (warps of one kernel, CTAs of the other): whatever the lengths of the requests, no slot has more to
 // do than another.  A cut inside a job leaves partial results, which are joined; slot c works from starts[c] to starts[c + 1].
 constexpr int PG_ROWS = 16, PG_KEYS = 16, PG_SLOTS = 1184;
-// Requests of up to so many rows per key head go to the kernel for few rows.  us, few rows / tiles: 16 requests behind 300 to 5 000 tokens, 32 heads
-// over 8, 20 rows 51 / 57, 32 rows 57 / 60, 40 rows 71 / 61, heads of 64 38 / 43, 43 / 43, 54 / 43; one request behind 3 000 25 / 31, 25 / 34, 25 / 34.  A key
-// head of its own for every head is another matter, there is twice the cache to read for two tiles: 20 rows 166 / 150, 32 rows 176 / 119.
+// Requests of up to so many rows per key head go to the kernel for few rows.  us, few rows / tiles (inside a graph, four sets of inputs in turn): 16 requests
+// behind 300 to 5 000 tokens, 32 heads over 8, 20 rows 39 / 45, 32 rows 41 / 46, 40 rows 53 / 48, heads of 64 31 / 36, 32 / 36, 42 / 37; one request behind
+// 3 000 13 / 20, 13 / 19, 19 / 20.  A key head of its own for every head is another matter, there is twice the cache to read for two tiles: 16 rows
+// 79 / 138, 20 rows 135 / 137, 32 rows 140 / 113.
 inline __host__ __device__ int pg_few(int group) { return group > 1 ? 32 : PG_ROWS; }
 constexpr int PG_TILE = 256, PG_TILE_KEYS = 128, PG_TILE_SLOTS = 148;
 inline __host__ __device__ int pg_begin(int kind) { return kind ? 2 : 1; }

@@ -13,11 +13,12 @@
 // CTAs stay for the whole launch and take whole jobs, or equal shares of all (paged_plan); cut jobs leave partial results, which
 // join_kernel adds up.  Every wait is bounded.
 //
-// 512 tokens behind 30 000, 64 heads over 8 of 128, bf16: 452 us inside a graph, 1 124 TFLOP/s; 2 047 tokens of 32 heads 49 us; twelve prompts of 90 to
-// 3 000 tokens 157 us.  Bound by the chain of a block (scores, maximum, weights, products; 3 450 cycles for two sides that take turns, of
-// which the tensor cores are busy for 58 %) and the clock under this load: without the exponentials it takes 440 us, with next to no MMAs
-// 377, with neither 298.  Measured against this form, us: MMAs behind `lane == 0` 565, two threads per row 473, an MMA warp per side 505 (both
-// sides then fall into step), scores of 64 keys in two buffers 510, a quarter of the exponentials on the FMA units 468.
+// 512 tokens behind 30 000, 64 heads over 8 of 128, bf16: 459 us in a graph that runs for some milliseconds (1 107 TFLOP/s), 529 us when
+// called without a pause, under the power limit (960); 2 047 tokens of 32 heads 50 and 53 us, twelve prompts of 90 to 3 000 tokens 156 and
+// 167 us.  Bound by the chain of a block (scores, maximum, weights, products; 3 450 cycles for two sides that take turns, of which the tensor
+// cores are busy for 58 %) and the clock under this load: without the exponentials it takes 440 us, with next to no MMAs 377, with neither
+// 298.  Measured against this form (452 to 466 us then, all in short graphs): MMAs behind `lane == 0` 565, two threads per row 473, an MMA warp
+// per side 505 (both sides then fall into step), scores of 64 keys in two buffers 510, a quarter of the exponentials on the FMA units 468.
 #include <mutex>
 
 #include "../tcgen05.cuh"

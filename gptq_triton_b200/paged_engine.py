@@ -40,7 +40,7 @@ class _Request:
 
 
 class PagedEngine:
-	"""pages: of page_size tokens each, shared by all requests.  requests: how many may run at once.  max_seq: longest request, its generated
+	"""pages: of page_size tokens each (8, 16, 32, 64 or a multiple of 128: see paged.py), shared by all requests.  requests: how many may run at once.  max_seq: longest request, its generated
 	tokens included (rotary tables, columns of the block table).  portion: prompt tokens per step; longer prompts take several steps, in which the
 	others go on decoding."""
 
