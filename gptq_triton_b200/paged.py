@@ -11,7 +11,7 @@ request r behind past[r] cached ones
 
 Rows are the new tokens, request after request.  Lengths stay on the device: a captured graph serves whatever they are at its replay.
 The operators raise on arguments that the host can judge; what only the device sees (a page that does not exist, no pages left) sets
-the status word (_lib.kernel_status(): 4, 8) and touches no memory that is not its own; the results of such a step are not to be used.
+the status word (_lib.kernel_status(): 4, 8, 16) and touches no memory that is not its own; the results of such a step are not to be used.
 There is no gradient.
 
 Any page and any head size that is a multiple of 8 is served, but chunks run on tensor memory (several times faster) only in 16 bits, in heads

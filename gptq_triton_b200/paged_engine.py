@@ -40,9 +40,9 @@ class _Request:
 
 
 class PagedEngine:
-	"""pages: of page_size tokens each (8, 16, 32, 64 or a multiple of 128: see paged.py), shared by all requests.  requests: how many may run at once.  max_seq: longest request, its generated
-	tokens included (rotary tables, columns of the block table).  portion: prompt tokens per step; longer prompts take several steps, in which the
-	others go on decoding."""
+	"""pages: of page_size tokens each, shared by all requests (prompts are fastest in pages of 8, 16, 32, 64 or a multiple of 128).  requests: how many
+	may run at once.  max_seq: longest request, its generated tokens included (rotary tables, columns of the block table).  portion: prompt
+	tokens per step; longer prompts take several steps, in which the others go on decoding."""
 
 	def __init__(self, model, pages: int, page_size: int = 16, requests: int = 16, max_seq: Optional[int] = None, portion: int = 2048, use_graph: bool = True):
 		if getattr(model, 'tp_world', 1) != 1:
